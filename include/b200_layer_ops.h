@@ -9,7 +9,8 @@
  * Part 2 declares what the reference does elsewhere than in a launcher of its own (bf16 rows, the q/k norm + RoPE and
  * the KV-cache row writes it runs inside attn_prep, the embedding decode it runs in a host loop, the FP16 component
  * kernels it launches by name) and is additive. Part 3: the same operations on host buffers, streamed through one or
- * several GPUs. Part 4: reading a GGUF file's tensor table and uploading a tensor.
+ * several GPUs. Part 4: reading a GGUF file's tensor table and uploading a tensor. Part 5: attention over the prepared
+ * rows and over a paged cache, and the pages of that cache.
  *
  * Conventions, all from the reference (src/gpu_ops.h:1-2, src/gpu_ops.cpp:66-86): every pointer is device memory
  * owned by the caller unless a parameter says "host"; launches are asynchronous on `stream` and never synchronise;
@@ -500,6 +501,85 @@ long long b200_gguf_kv_str(const b200_gguf* g, const char* key, char* buf, size_
  * returns the device pointer; release it with b200_gguf_free_tensor. The mapping must stay open until the copy ran. */
 cudaError_t b200_gguf_upload_tensor(const b200_gguf* g, int idx, void** dev_ptr, cudaStream_t stream);
 void b200_gguf_free_tensor(void* dev_ptr);
+
+/* ------------------------------------------------------------------------------------------------ Part 5 */
+
+/* Attention over the rows that parts 1 and 2 prepare, and the pages of a cache that many sequences share. The
+ * reference's own attention (attn_partial_*, attn_flash_*, src/attention.hip) serves one sequence; these calls are
+ * additive. head_dim is 64, 128 or 256; n_q is a multiple of n_kv, query head h reads key head h / (n_q / n_kv); scale
+ * is finite and greater than 0. Scores, softmax and sums are held in fp32. These launchers look at their arguments first:
+ * what the contract forbids is cudaErrorInvalidValue with or without a device.
+ *
+ * Causal attention over packed prompts: sequence b is rows seq_start[b] .. seq_start[b + 1] - 1 of the T rows
+ * (seq_start: n_seqs + 1 ascending ints in device memory; NULL: the T rows are one sequence, n_seqs 1), and row t sees
+ * the rows of its own sequence up to itself:
+ *   out[t][h] = sum_j p_j v[j][h / G] / sum_j p_j,  p_j = exp(scale * q[t][h] . k[j][h / G])
+ * q [T][n_q * head_dim] as gpu_qk_norm_rope leaves it, k and v [T][n_kv * head_dim], bf16 or fp16 bit patterns; rows may
+ * sit q_stride / k_stride / v_stride values apart (multiples of 8; 0: contiguous), e.g. in a fused q | k | v
+ * projection. out [T][n_q * head_dim] is contiguous and shares no memory with the inputs. Empty sequences are
+ * allowed; rows before the first and behind the last sequence are neither read into a result nor written. Weights are
+ * rounded to the rows' type before they meet v (the sum of weights is not), out once. T <= 2^30; pointers 16-byte
+ * aligned. */
+cudaError_t gpu_attn_prompt_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int* seq_start,
+                                 int n_seqs, long long T, int n_q, int n_kv, int head_dim, long long q_stride, long long k_stride,
+                                 long long v_stride, float scale, cudaStream_t stream);
+cudaError_t gpu_attn_prompt_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int* seq_start,
+                                int n_seqs, long long T, int n_q, int n_kv, int head_dim, long long q_stride, long long k_stride,
+                                long long v_stride, float scale, cudaStream_t stream);
+
+/* Attention of one token per sequence over a paged FP16 cache: q, out [B][n_q * head_dim]; sequence b sees its first
+ * lens[b] cache rows (its own token's row included, once stored). Row t of sequence b is row t mod 2^kv_shift of page
+ * pages[b][t >> kv_shift] (pages: [B][max_pages] ints), and row r of page p is at K + p * kv_bstride + r * kv_stride
+ * values, V likewise: the block-major cache that gpu_kv_store_f16 writes, with positions = p * 2^kv_shift + r. Ids outside
+ * [0, n_pages) are rows that are not seen. lens[b] <= 0: out[b] is zero.
+ * prefix_len > 0: every sequence with lens[b] >= prefix_len begins with the same prefix_len rows IN THE SAME PAGES (as
+ * gpu_kv_pages_fork leaves them), which are then read once for the whole batch; a multiple of 2^kv_shift. Sequences with
+ * fewer rows (idle slots) use their own pages only. Memory behind lens[b] may hold anything.
+ * fp32 rows keep fp32 accuracy; kv_stride and kv_bstride are multiples of 8, pointers 16-byte aligned, out is not q.
+ * scratch: device memory of gpu_attn_decode_scratch_bytes(...) bytes, any contents, in use until the call has run; calls
+ * that may overlap need scratch of their own. */
+size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len);
+cudaError_t gpu_attn_decode(const float* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,
+                            int n_pages, const int* pages, int max_pages, const int* lens, int prefix_len, float* out, int n_q,
+                            int n_kv, int head_dim, int B, float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream);
+cudaError_t gpu_attn_decode_bf16(const uint16_t* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift,
+                                 long long kv_bstride, int n_pages, const int* pages, int max_pages, const int* lens, int prefix_len,
+                                 uint16_t* out, int n_q, int n_kv, int head_dim, int B, float scale, void* scratch,
+                                 size_t scratch_bytes, cudaStream_t stream);
+
+/* The pages of such a cache. The caller owns every array (device memory) and starts with lens and refs all 0; the calls
+ * below keep them consistent. A page is free when its count is 0; the lowest free ids are taken first, sequences in
+ * ascending order, so equal calls give equal tables. A page's bytes lie at pool + i * part_stride + page * page_bytes for
+ * i < n_parts: one part for a block-major pool (page_bytes = 2 * kv_bstride), or one per layer and K / V half.
+ * Every call writes info: [0] 0 (done), 1 (too few free pages), 2 (an argument in device memory is not allowed), [1] free
+ * pages afterwards, [2] pages copied. Calls on one b200_kv_pages are ordered by the caller (one stream). */
+typedef struct b200_kv_pages {
+    int* table;          /* [n_seqs][max_pages] page ids; entries behind a sequence's last page are -1 or never used */
+    int* lens;           /* [n_seqs] rows */
+    int* refs;           /* [n_pages] sequences that hold the page */
+    int* info;           /* [4] */
+    int* work;           /* gpu_kv_pages_work_ints(n_seqs, n_pages) ints, any contents */
+    int n_seqs, max_pages, n_pages;
+    int page_shift;      /* a page holds 2^page_shift rows; n_pages << page_shift fits an int */
+    void* pool;          /* 16-byte aligned; page_bytes and part_stride multiples of 16 */
+    size_t page_bytes;
+    int n_parts;
+    size_t part_stride;  /* >= n_pages * page_bytes when n_parts > 1 */
+} b200_kv_pages;
+size_t gpu_kv_pages_work_ints(int n_seqs, int n_pages);
+/* parent [n_seqs]: -1, or the sequence that the so far empty sequence s becomes a copy of. Whole pages are shared; a last
+ * page that is partly filled is copied, so that parent and copy may both grow. Nothing changes unless info[0] is 0 (2: a
+ * parent out of range or s itself, or s not empty). */
+cudaError_t gpu_kv_pages_fork(const b200_kv_pages* kv, const int* parent, cudaStream_t stream);
+/* new_lens [n_seqs]: the length sequence s gets (0 frees it, < 0 keeps it). Shorter sequences give their pages back first;
+ * then the longer ones take the pages they lack. A partly filled last page that another sequence shares (both were cut
+ * back into it) is replaced by a copy before it grows. slots (NULL: none): the cache rows page * 2^page_shift + row of the
+ * new tokens, sequence after sequence, what gpu_kv_store_f16 takes as positions; n_slots: how many fit. If the pages do not
+ * suffice (1) or a length exceeds the table (2) no sequence grows and slots stays as it was. new_lens is not lens. */
+cudaError_t gpu_kv_pages_resize(const b200_kv_pages* kv, const int* new_lens, int* slots, int n_slots, cudaStream_t stream);
+/* Moves the pages in use to the front: those at or behind n_live = n_pages - (free pages) go, in ascending order, to the
+ * free ids before it; tables and counts follow. Source pages keep their bytes. */
+cudaError_t gpu_kv_pages_compact(const b200_kv_pages* kv, cudaStream_t stream);
 
 /* Number of kernel launches this library has issued since it was loaded (all launchers, all threads) */
 unsigned long long b200_launch_count(void);

@@ -38,6 +38,14 @@ class b200_layer_sweep(C.Structure):
     ]
 
 
+class b200_kv_pages(C.Structure):
+    """Layout of struct b200_kv_pages (include/b200_layer_ops.h): page tables, counts and the pool they speak of."""
+    _fields_ = [
+        ("table", _p), ("lens", _p), ("refs", _p), ("info", _p), ("work", _p), ("n_seqs", _i), ("max_pages", _i), ("n_pages", _i),
+        ("page_shift", _i), ("pool", _p), ("page_bytes", _sz), ("n_parts", _i), ("part_stride", _sz),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/b200_layer_ops.h declares
 SIGNATURES = {
     "gpu_ops_init": (_i, [C.c_char_p]),
@@ -129,6 +137,15 @@ SIGNATURES = {
     "b200_gguf_kv_str": (_ll, [_p, C.c_char_p, C.c_char_p, _sz]),
     "b200_gguf_upload_tensor": (_i, [_p, _i, C.POINTER(_p), _p]),
     "b200_gguf_free_tensor": (None, [_p]),
+    "gpu_attn_prompt_bf16": (_i, [_p, _p, _p, _p, _p, _i, _ll, _i, _i, _i, _ll, _ll, _ll, _f, _p]),
+    "gpu_attn_prompt_f16": (_i, [_p, _p, _p, _p, _p, _i, _ll, _i, _i, _i, _ll, _ll, _ll, _f, _p]),
+    "gpu_attn_decode_scratch_bytes": (_sz, [_i, _i, _i, _i, _i]),
+    "gpu_attn_decode": (_i, [_p, _p, _p, _i, _i, _ll, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _f, _p, _sz, _p]),
+    "gpu_attn_decode_bf16": (_i, [_p, _p, _p, _i, _i, _ll, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _f, _p, _sz, _p]),
+    "gpu_kv_pages_work_ints": (_sz, [_i, _i]),
+    "gpu_kv_pages_fork": (_i, [C.POINTER(b200_kv_pages), _p, _p]),
+    "gpu_kv_pages_resize": (_i, [C.POINTER(b200_kv_pages), _p, _p, _i, _p]),
+    "gpu_kv_pages_compact": (_i, [C.POINTER(b200_kv_pages), _p]),
     "b200_launch_count": (C.c_ulonglong, []),
     "b200_build_arch": (C.c_char_p, []),
 }

@@ -1,0 +1,171 @@
+// attention.cu -- launchers of part 5 of include/b200_layer_ops.h: attention over packed prompts, attention of single
+// tokens over a paged cache, and the pages of that cache.
+
+#include "b200_layer_ops.h"
+
+#include <limits.h>
+#include <math.h>
+
+#include <type_traits>
+
+#include "attn_decode.cuh"
+#include "attn_prompt.cuh"
+#include "internal.h"
+#include "kv_pages.cuh"
+#include "launch.cuh"
+
+using namespace b200;
+
+namespace {
+
+bool good_scale(float s) { return s > 0.0f && s < INFINITY; }
+bool good_heads(int n_q, int n_kv, int D) {
+    return n_q > 0 && n_kv > 0 && n_q % n_kv == 0 && (D == 64 || D == 128 || D == 256) && n_q <= INT_MAX / D;
+}
+
+// ---------------------------------------------------------------- prompts
+
+template <typename T>
+cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int* seq_start, int n_seqs, long long rows, int n_q,
+                          int n_kv, int D, long long q_stride, long long k_stride, long long v_stride, float scale,
+                          cudaStream_t stream) {
+    if (!q || !k || !v || !out || n_seqs < 1 || (!seq_start && n_seqs != 1) || rows < 1 || rows > (1 << 30) ||
+        !good_heads(n_q, n_kv, D) || !good_scale(scale))
+        return cudaErrorInvalidValue;
+    if (q_stride == 0) q_stride = (long long)n_q * D;
+    if (k_stride == 0) k_stride = (long long)n_kv * D;
+    if (v_stride == 0) v_stride = (long long)n_kv * D;
+    if (q_stride < (long long)n_q * D || k_stride < (long long)n_kv * D || v_stride < (long long)n_kv * D || q_stride % 8 ||
+        k_stride % 8 || v_stride % 8 || !al16(q) || !al16(k) || !al16(v) || !al16(out) || out == q || out == k || out == v)
+        return cudaErrorInvalidValue;
+    const long long grid = (rows * n_q + 3) / 4;
+    if (grid > INT_MAX) return cudaErrorInvalidValue;
+    if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
+#define ROWS(D_) launch_pdl((k_attn_prompt_rows<D_, T>), (unsigned)grid, 128, 0, stream, q, k, v, out, seq_start, n_seqs, (int)rows, \
+                            n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E)
+    if (D == 64) ROWS(64); else if (D == 128) ROWS(128); else ROWS(256);
+#undef ROWS
+    return launched();
+}
+
+// ---------------------------------------------------------------- single tokens
+
+template <typename T>
+cudaError_t launch_decode(const T* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,
+                          int n_pages, const int* pages, int max_pages, const int* lens, int prefix_len, T* out, int n_q, int n_kv,
+                          int D, int B, float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+    if (!q || !K || !V || !pages || !lens || !out || !good_heads(n_q, n_kv, D) || !good_scale(scale) || B < 1 || n_pages < 1 ||
+        max_pages < 1 || kv_shift < 0 || kv_shift > 30 || kv_stride < (long long)n_kv * D || kv_stride % 8 || kv_bstride % 8 ||
+        kv_bstride < 0 || !al16(q) || !al16(K) || !al16(V) || !al16(out) || (const void*)out == (const void*)q)
+        return cudaErrorInvalidValue;
+    if (prefix_len < 0 || prefix_len % (1 << kv_shift) || prefix_len > ((long long)max_pages << kv_shift)) return cudaErrorInvalidValue;
+    const size_t need = gpu_attn_decode_scratch_bytes(n_q, n_kv, D, B, prefix_len);
+    if (need == 0 || scratch_bytes < need || !scratch || !al16(scratch)) return cudaErrorInvalidValue;
+    if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
+    const PagedKv kv{reinterpret_cast<const __half*>(K), reinterpret_cast<const __half*>(V), pages, lens, kv_bstride, kv_stride,
+                     kv_shift, n_pages, max_pages};
+    const long long grid = ((long long)B * n_q + 3) / 4;
+#define ROWS(D_) launch_pdl((k_attn_decode_rows<D_, T>), (unsigned)grid, 128, 0, stream, q, kv, out, n_q, n_q / n_kv, B, scale * LOG2E)
+    if (D == 64) ROWS(64); else if (D == 128) ROWS(128); else ROWS(256);
+#undef ROWS
+    return launched();
+}
+
+// ---------------------------------------------------------------- pages
+
+bool good_pages(const b200_kv_pages* kv) {
+    return kv && kv->table && kv->lens && kv->refs && kv->info && kv->work && kv->pool && kv->n_seqs > 0 && kv->max_pages > 0 &&
+           kv->n_pages > 0 && kv->page_shift >= 0 && kv->page_shift <= 30 &&
+           ((long long)kv->n_pages << kv->page_shift) <= INT_MAX && kv->page_bytes > 0 && kv->page_bytes % 16 == 0 &&
+           kv->page_bytes <= INT_MAX && kv->n_parts > 0 && (kv->n_parts == 1 || kv->part_stride >= kv->page_bytes * kv->n_pages) &&
+           kv->part_stride % 16 == 0 && al16(kv->pool) && (long long)kv->n_seqs * kv->max_pages <= (1LL << 40);
+}
+
+// The control kernel as one cluster, then the copies it listed
+template <typename... KA, typename... A>
+cudaError_t launch_pages(const b200_kv_pages* kv, cudaStream_t stream, void (*kernel)(KA...), A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(KVP_CTAS, 1, 1);
+    cfg.blockDim = dim3(KVP_THREADS, 1, 1);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = KVP_CTAS;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<KA>(args)...);
+    const cudaError_t st = launched();
+    if (st != cudaSuccess) return st;
+    launch_pdl(k_kv_pages_copy, (unsigned)resident_ctas(256), 256, 0, stream, *kv);
+    return launched();
+}
+
+}  // namespace
+
+extern "C" {
+
+cudaError_t gpu_attn_prompt_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int* seq_start,
+                                 int n_seqs, long long T, int n_q, int n_kv, int head_dim, long long q_stride, long long k_stride,
+                                 long long v_stride, float scale, cudaStream_t stream) {
+    using E = __nv_bfloat16;
+    return launch_prompt(reinterpret_cast<const E*>(q), reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v),
+                         reinterpret_cast<E*>(out), seq_start, n_seqs, T, n_q, n_kv, head_dim, q_stride, k_stride, v_stride, scale,
+                         stream);
+}
+
+cudaError_t gpu_attn_prompt_f16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int* seq_start,
+                                int n_seqs, long long T, int n_q, int n_kv, int head_dim, long long q_stride, long long k_stride,
+                                long long v_stride, float scale, cudaStream_t stream) {
+    using E = __half;
+    return launch_prompt(reinterpret_cast<const E*>(q), reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v),
+                         reinterpret_cast<E*>(out), seq_start, n_seqs, T, n_q, n_kv, head_dim, q_stride, k_stride, v_stride, scale,
+                         stream);
+}
+
+size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len) {
+    if (!good_heads(n_q, n_kv, head_dim) || B < 1 || prefix_len < 0) return 0;
+    return 256;
+}
+
+cudaError_t gpu_attn_decode(const float* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,
+                            int n_pages, const int* pages, int max_pages, const int* lens, int prefix_len, float* out, int n_q,
+                            int n_kv, int head_dim, int B, float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
+    return launch_decode(q, K, V, kv_stride, kv_shift, kv_bstride, n_pages, pages, max_pages, lens, prefix_len, out, n_q, n_kv,
+                         head_dim, B, scale, scratch, scratch_bytes, stream);
+}
+
+cudaError_t gpu_attn_decode_bf16(const uint16_t* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift,
+                                 long long kv_bstride, int n_pages, const int* pages, int max_pages, const int* lens, int prefix_len,
+                                 uint16_t* out, int n_q, int n_kv, int head_dim, int B, float scale, void* scratch,
+                                 size_t scratch_bytes, cudaStream_t stream) {
+    return launch_decode(reinterpret_cast<const __nv_bfloat16*>(q), K, V, kv_stride, kv_shift, kv_bstride, n_pages, pages, max_pages,
+                         lens, prefix_len, reinterpret_cast<__nv_bfloat16*>(out), n_q, n_kv, head_dim, B, scale, scratch,
+                         scratch_bytes, stream);
+}
+
+size_t gpu_kv_pages_work_ints(int n_seqs, int n_pages) {
+    return n_seqs > 0 && n_pages > 0 ? KvPagesWork::ints(n_seqs, n_pages) : 0;
+}
+
+cudaError_t gpu_kv_pages_fork(const b200_kv_pages* kv, const int* parent, cudaStream_t stream) {
+    if (!good_pages(kv) || !parent || parent == kv->lens) return cudaErrorInvalidValue;
+    if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
+    return launch_pages(kv, stream, k_kv_pages_fork, *kv, parent);
+}
+
+cudaError_t gpu_kv_pages_resize(const b200_kv_pages* kv, const int* new_lens, int* slots, int n_slots, cudaStream_t stream) {
+    if (!good_pages(kv) || !new_lens || new_lens == kv->lens || n_slots < 0) return cudaErrorInvalidValue;
+    if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
+    return launch_pages(kv, stream, k_kv_pages_resize, *kv, new_lens, slots, n_slots);
+}
+
+cudaError_t gpu_kv_pages_compact(const b200_kv_pages* kv, cudaStream_t stream) {
+    if (!good_pages(kv)) return cudaErrorInvalidValue;
+    if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
+    return launch_pages(kv, stream, k_kv_pages_compact, *kv);
+}
+
+}  // extern "C"

@@ -14,6 +14,8 @@ from . import _lib
 __all__ = [
     "LayerOpError", "gpu_ops_init", "gpu_ops_free", "gpu_add_rmsnorm", "gpu_swiglu", "gpu_swiglu_rows",
     "gpu_qk_norm_rope", "gpu_rope_table", "gpu_qk_norm_rope_tab", "gpu_qk_norm_rope_tab_kv", "gpu_qk_norm_rope_kv", "gpu_attn_prep_f16", "gpu_embed_rows", "gpu_moe_group", "gpu_moe_group_scratch_ints", "gpu_moe_max_tiles", "gpu_kv_store_f16", "gpu_kv_store_q", "gpu_hadamard_rot", "gpu_add_normed", "gpu_gemma_attn_post", "gpu_geglu", "gpu_softcap", "gpu_gemma_ffn_post", "gpu_moe_combine", "gpu_moe_router", "gpu_moe_router_sigmoid", "gpu_relu2", "gpu_mamba_conv", "gpu_mamba_scan", "gpu_ple_conv", "gpu_hc_norm", "gpu_hc_lowrank", "gpu_hc_mix", "gpu_ple_gate", "gpu_mtp_concat", "gpu_mamba_gnorm", "gpu_rmsnorm_f16", "gpu_rope_rotate_half_f16", "launch_count", "Q8Buffers",
+    "gpu_attn_prompt", "gpu_attn_decode", "gpu_attn_decode_scratch_bytes", "KvPages", "gpu_kv_pages_fork",
+    "gpu_kv_pages_resize", "gpu_kv_pages_compact",
     "QT_Q4_0", "QT_Q8_0", "QT_F32", "QT_F16", "QT_BF16", "QT_Q4_1", "QT_Q5_0", "QT_Q5_1", "QT_Q4_K", "QT_Q5_K", "QT_Q6_K",
     "QT_BLOCKS", "qt_row_size", "HostRows", "HostGroup",
 ]
@@ -388,6 +390,76 @@ def gpu_rmsnorm_f16(x, gamma, y, n_tokens, n_embd, eps):
 def gpu_rope_rotate_half_f16(x, ctab, stab, y, n_rows, half_dim):
     _check("gpu_rope_rotate_half_f16",
            _lib.load().gpu_rope_rotate_half_f16(_ptr(x), _ptr(ctab), _ptr(stab), _ptr(y), n_rows, half_dim, _stream()))
+
+
+def gpu_attn_prompt(q, k, v, out, seq_start, n_seqs, T, n_q, n_kv, head_dim, scale, q_stride=0, k_stride=0, v_stride=0):
+    """Causal attention over packed prompts: sequence b is rows seq_start[b] .. seq_start[b + 1] - 1 (int32 CUDA tensor of
+    n_seqs + 1 entries; None: one sequence of T rows). q, k, v, out: bfloat16 or float16 CUDA tensors."""
+    if q.dtype not in (torch.bfloat16, torch.float16) or not (q.dtype == k.dtype == v.dtype == out.dtype):
+        raise TypeError((q.dtype, k.dtype, v.dtype, out.dtype))
+    lib = _lib.load()
+    fn = lib.gpu_attn_prompt_bf16 if q.dtype == torch.bfloat16 else lib.gpu_attn_prompt_f16
+    _check("gpu_attn_prompt", fn(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(seq_start), n_seqs, T, n_q, n_kv, head_dim, q_stride,
+                                 k_stride, v_stride, scale, _stream()))
+
+
+def gpu_attn_decode_scratch_bytes(n_q, n_kv, head_dim, B, prefix_len=0):
+    return int(_lib.load().gpu_attn_decode_scratch_bytes(n_q, n_kv, head_dim, B, prefix_len))
+
+
+def gpu_attn_decode(q, K, V, kv_stride, kv_shift, kv_bstride, n_pages, pages, max_pages, lens, prefix_len, out, n_q, n_kv,
+                    head_dim, B, scale, scratch=None):
+    """Attention of one token per sequence over the paged FP16 cache K / V (float16 CUDA tensors, row 0 of page 0 of the
+    layer's K and V). q, out: float32 or bfloat16 [B][n_q * head_dim]; pages int32 [B][max_pages]; lens int32 [B];
+    prefix_len: rows that all sequences share, read once. scratch: a CUDA tensor of gpu_attn_decode_scratch_bytes(...)
+    bytes (one is made when None)."""
+    if q.dtype not in (torch.float32, torch.bfloat16) or q.dtype != out.dtype or K.dtype != torch.float16 or V.dtype != torch.float16:
+        raise TypeError((q.dtype, out.dtype, K.dtype, V.dtype))
+    lib = _lib.load()
+    if scratch is None:
+        scratch = torch.empty(gpu_attn_decode_scratch_bytes(n_q, n_kv, head_dim, B, prefix_len), dtype=torch.uint8, device=q.device)
+    fn = lib.gpu_attn_decode if q.dtype == torch.float32 else lib.gpu_attn_decode_bf16
+    _check("gpu_attn_decode", fn(_ptr(q), _ptr(K), _ptr(V), kv_stride, kv_shift, kv_bstride, n_pages, _ptr(pages), max_pages, _ptr(lens),
+                                 prefix_len, _ptr(out), n_q, n_kv, head_dim, B, scale, _ptr(scratch),
+                                 scratch.numel() * scratch.element_size(), _stream()))
+
+
+class KvPages:
+    """The page tables of a paged cache and its pool (struct b200_kv_pages): table int32 [n_seqs][max_pages], lens int32
+    [n_seqs], refs int32 [n_pages], info int32 [4], all CUDA tensors, lens and refs zero to begin with; pool: a CUDA tensor
+    whose part i holds page p at byte i * part_stride + p * page_bytes."""
+
+    def __init__(self, table, lens, refs, info, page_shift, pool, page_bytes, n_parts=1, part_stride=0):
+        n_seqs, max_pages = table.shape
+        for t, n in ((table, n_seqs * max_pages), (lens, n_seqs), (refs, refs.numel()), (info, 4)):
+            assert t.is_cuda and t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n
+        n_pages = refs.numel()
+        assert pool.is_cuda and pool.numel() * pool.element_size() >= (n_parts - 1) * part_stride + n_pages * page_bytes
+        self.work = torch.empty(int(_lib.load().gpu_kv_pages_work_ints(n_seqs, n_pages)), dtype=torch.int32, device=table.device)
+        self.table, self.lens, self.refs, self.info, self.pool = table, lens, refs, info, pool
+        p = lambda t: t.data_ptr()  # noqa: E731
+        self._struct = _lib.b200_kv_pages(p(table), p(lens), p(refs), p(info), p(self.work), n_seqs, max_pages, n_pages, page_shift,
+                                          p(pool), page_bytes, n_parts, part_stride)
+
+    def struct(self):
+        return self._struct
+
+
+def gpu_kv_pages_fork(kv, parent):
+    """parent int32 [n_seqs]: -1, or the sequence that the empty sequence s becomes a copy of."""
+    _check("gpu_kv_pages_fork", _lib.load().gpu_kv_pages_fork(C.byref(kv.struct()), _ptr(parent), _stream()))
+
+
+def gpu_kv_pages_resize(kv, new_lens, slots=None):
+    """new_lens int32 [n_seqs]: the length each sequence gets (0 frees it, negative keeps it); slots (int32): receives the
+    cache rows of the new tokens."""
+    _check("gpu_kv_pages_resize", _lib.load().gpu_kv_pages_resize(C.byref(kv.struct()), _ptr(new_lens), _ptr(slots),
+                                                                  0 if slots is None else slots.numel(), _stream()))
+
+
+def gpu_kv_pages_compact(kv):
+    """Moves the pages in use to the lowest ids."""
+    _check("gpu_kv_pages_compact", _lib.load().gpu_kv_pages_compact(C.byref(kv.struct()), _stream()))
 
 
 class HostRows:
