@@ -527,6 +527,11 @@ cudaError_t gpu_attn_prompt_f16(const uint16_t* q, const uint16_t* k, const uint
                                 int n_seqs, long long T, int n_q, int n_kv, int head_dim, long long q_stride, long long k_stride,
                                 long long v_stride, float scale, cudaStream_t stream);
 
+/* The attention kernels wait for their own copies and products with a limit on every wait; a block that gives up leaves its
+ * rows unspecified and ends. How many did on the current device since the library was loaded (waits for the device;
+ * -1: not available): 0 in sound operation. */
+int b200_attn_gave_up(void);
+
 /* Attention of one token per sequence over a paged FP16 cache: q, out [B][n_q * head_dim]; sequence b sees its first
  * lens[b] cache rows (its own token's row included, once stored). Row t of sequence b is row t mod 2^kv_shift of page
  * pages[b][t >> kv_shift] (pages: [B][max_pages] ints), and row r of page p is at K + p * kv_bstride + r * kv_stride

@@ -139,6 +139,7 @@ SIGNATURES = {
     "b200_gguf_free_tensor": (None, [_p]),
     "gpu_attn_prompt_bf16": (_i, [_p, _p, _p, _p, _p, _i, _ll, _i, _i, _i, _ll, _ll, _ll, _f, _p]),
     "gpu_attn_prompt_f16": (_i, [_p, _p, _p, _p, _p, _i, _ll, _i, _i, _i, _ll, _ll, _ll, _f, _p]),
+    "b200_attn_gave_up": (_i, []),
     "gpu_attn_decode_scratch_bytes": (_sz, [_i, _i, _i, _i, _i]),
     "gpu_attn_decode": (_i, [_p, _p, _p, _i, _i, _ll, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _f, _p, _sz, _p]),
     "gpu_attn_decode_bf16": (_i, [_p, _p, _p, _i, _i, _ll, _i, _p, _i, _p, _i, _p, _i, _i, _i, _i, _f, _p, _sz, _p]),

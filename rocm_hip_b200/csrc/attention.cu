@@ -6,6 +6,10 @@
 #include <limits.h>
 #include <math.h>
 
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
 #include <type_traits>
 
 #include "attn_decode.cuh"
@@ -23,6 +27,48 @@ bool good_heads(int n_q, int n_kv, int D) {
     return n_q > 0 && n_kv > 0 && n_q % n_kv == 0 && (D == 64 || D == 128 || D == 256) && n_q <= INT_MAX / D;
 }
 
+// ---------------------------------------------------------------- tensor maps
+
+// cuTensorMapEncodeTiled by the runtime's entry point lookup: the library does not link the driver
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+    static std::atomic<PFN_cuTensorMapEncodeTiled_v12000> cached{nullptr};
+    PFN_cuTensorMapEncodeTiled_v12000 fn = cached.load(std::memory_order_acquire);
+    if (!fn) {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            (void)cudaGetLastError();
+            return nullptr;
+        }
+        fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+        cached.store(fn, std::memory_order_release);
+    }
+    return fn;
+}
+
+template <typename T>
+constexpr CUtensorMapDataType map_type() {
+    return std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+}
+
+// rows [T][heads * D] `stride` values apart, fetched as boxes of 128 rows x 64 values of one head
+template <typename T>
+bool row_map(CUtensorMap* m, const T* p, int D, int heads, long long rows, long long stride) {
+    const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {CHUNK, 1, TILE_ROWS}, step[3] = {1, 1, 1};
+    const auto fn = encode_fn();
+    return fn && fn(m, map_type<T>(), 3, const_cast<T*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Lets the kernel have `bytes` of dynamic shared memory on the current device
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes) {
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 // ---------------------------------------------------------------- prompts
 
 template <typename T>
@@ -38,13 +84,25 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
     if (q_stride < (long long)n_q * D || k_stride < (long long)n_kv * D || v_stride < (long long)n_kv * D || q_stride % 8 ||
         k_stride % 8 || v_stride % 8 || !al16(q) || !al16(k) || !al16(v) || !al16(out) || out == q || out == k || out == v)
         return cudaErrorInvalidValue;
-    const long long grid = (rows * n_q + 3) / 4;
+    const int per = D == 256 ? PromptShape<256>::ROWS : PromptShape<128>::ROWS;
+    const long long n_slots = seq_start ? rows / per + n_seqs : (rows + per - 1) / per, grid = n_slots * n_q;
     if (grid > INT_MAX) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
-#define ROWS(D_) launch_pdl((k_attn_prompt_rows<D_, T>), (unsigned)grid, 128, 0, stream, q, k, v, out, seq_start, n_seqs, (int)rows, \
-                            n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E)
-    if (D == 64) ROWS(64); else if (D == 128) ROWS(128); else ROWS(256);
-#undef ROWS
+    CUtensorMap mq, mk, mv;
+    if (!row_map<T>(&mq, q, D, n_q, rows, q_stride) || !row_map<T>(&mk, k, D, n_kv, rows, k_stride) ||
+        !row_map<T>(&mv, v, D, n_kv, rows, v_stride))
+        return cudaErrorInvalidValue;
+    cudaError_t st;
+#define TILES(D_)                                                                                                            \
+    do {                                                                                                                     \
+        st = allow_smem(k_attn_prompt<D_, T>, PromptShape<D_>::SMEM);                                                        \
+        if (st != cudaSuccess) return st;                                                                                    \
+        launch_pdl((k_attn_prompt<D_, T>), (unsigned)grid, PromptShape<D_>::WARPS * 32, PromptShape<D_>::SMEM, stream, mq, mk, mv, q, \
+                   k, v, out, seq_start, n_seqs, (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E,    \
+                   (int)n_slots);                                                                                            \
+    } while (0)
+    if (D == 64) TILES(64); else if (D == 128) TILES(128); else TILES(256);
+#undef TILES
     return launched();
 }
 
@@ -123,6 +181,11 @@ cudaError_t gpu_attn_prompt_f16(const uint16_t* q, const uint16_t* k, const uint
     return launch_prompt(reinterpret_cast<const E*>(q), reinterpret_cast<const E*>(k), reinterpret_cast<const E*>(v),
                          reinterpret_cast<E*>(out), seq_start, n_seqs, T, n_q, n_kv, head_dim, q_stride, k_stride, v_stride, scale,
                          stream);
+}
+
+int b200_attn_gave_up(void) {
+    int n = 0;
+    return cudaMemcpyFromSymbol(&n, attn_gave_up, sizeof n) == cudaSuccess ? n : -1;
 }
 
 size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len) {
