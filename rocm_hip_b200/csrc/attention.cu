@@ -13,6 +13,8 @@
 #include <type_traits>
 
 #include "attn_decode.cuh"
+#include "attn_own.cuh"
+#include "attn_prefix.cuh"
 #include "attn_prompt.cuh"
 #include "internal.h"
 #include "kv_pages.cuh"
@@ -84,7 +86,7 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
     if (q_stride < (long long)n_q * D || k_stride < (long long)n_kv * D || v_stride < (long long)n_kv * D || q_stride % 8 ||
         k_stride % 8 || v_stride % 8 || !al16(q) || !al16(k) || !al16(v) || !al16(out) || out == q || out == k || out == v)
         return cudaErrorInvalidValue;
-    const int per = D == 256 ? PromptShape<256>::ROWS : PromptShape<128>::ROWS;
+    const int per = prompt_rows(D);
     const long long n_slots = seq_start ? rows / per + n_seqs : (rows + per - 1) / per, grid = n_slots * n_q;
     if (grid > INT_MAX) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
@@ -95,11 +97,11 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
     cudaError_t st;
 #define TILES(D_)                                                                                                            \
     do {                                                                                                                     \
-        st = allow_smem(k_attn_prompt<D_, T>, PromptShape<D_>::SMEM);                                                        \
+        using Ti = PromptTiles<D_, T>;                                                                                       \
+        st = allow_smem(k_attn_prompt<D_, T>, Ti::SMEM);                                                                     \
         if (st != cudaSuccess) return st;                                                                                    \
-        launch_pdl((k_attn_prompt<D_, T>), (unsigned)grid, PromptShape<D_>::WARPS * 32, PromptShape<D_>::SMEM, stream, mq, mk, mv, q, \
-                   k, v, out, seq_start, n_seqs, (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E,    \
-                   (int)n_slots);                                                                                            \
+        launch_pdl((k_attn_prompt<D_, T>), (unsigned)grid, Ti::WARPS * 32, Ti::SMEM, stream, mq, mk, mv, q, k, v, out, seq_start, \
+                   n_seqs, (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E, (int)n_slots);           \
     } while (0)
     if (D == 64) TILES(64); else if (D == 128) TILES(128); else TILES(256);
 #undef TILES
@@ -108,25 +110,120 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
 
 // ---------------------------------------------------------------- single tokens
 
+// The pages of one half (K or V) of a layer, fetched as boxes of up to 128 rows x 64 values of one head
+bool page_map(CUtensorMap* m, const __half* p, int D, int heads, const PagedKv& kv) {
+    const int in_page = 1 << kv.kv_shift;
+    const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)in_page, (cuuint64_t)kv.n_pages};
+    const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)kv.kv_stride * 2,
+                                   (cuuint64_t)(kv.n_pages > 1 ? kv.kv_bstride : kv.kv_stride) * 2};
+    const cuuint32_t box[4] = {CHUNK, 1, (cuuint32_t)(in_page < TILE_ROWS ? in_page : TILE_ROWS), 1}, step[4] = {1, 1, 1, 1};
+    const auto fn = encode_fn();
+    return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(p), dims, strides, box, step,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// What a decode call launches and where its pieces lie in scratch: a function of the sizes the host knows
+struct DecodePlan {
+    int grid_own, nq, row_tiles, splits;     // splits 0: nothing is shared
+    long long px_rows;
+    size_t first, own_ml, own_o, px_ml, px_o, bytes;
+
+    DecodePlan(int n_q, int n_kv, int D, int B, int prefix) {
+        const int warps = D == 256 ? OwnShape<256>::WARPS : OwnShape<128>::WARPS, sms = sm_count();
+        const OwnPlan own(n_q, n_kv, warps);
+        grid_own = sms;
+        const size_t pieces = ((size_t)grid_own + (size_t)B * own.groups) * warps * own.hg;
+        splits = 0;
+        nq = row_tiles = 0;
+        px_rows = 0;
+        const long long M = (long long)B * (n_q / n_kv);
+        // One sequence shares nothing, and less than two tiles of rows are not worth a launch of their own
+        if (B > 1 && prefix >= 2 * TILE_ROWS) {
+            nq = D == 256 || M <= TILE_ROWS ? 1 : 2;
+            row_tiles = (int)((M + nq * TILE_ROWS - 1) / (nq * TILE_ROWS));
+            px_rows = (long long)row_tiles * nq * TILE_ROWS;
+            // stretches of the prefix: as many as make the CTAs whole waves of the device, counting about four tiles' time
+            // for what a CTA does once (its queries, its result and the pieces' way through scratch)
+            const int tiles = (prefix + TILE_ROWS - 1) / TILE_ROWS, base = n_kv * row_tiles;
+            long long best = LLONG_MAX;
+            for (int s = 1; s <= tiles && s <= 64; ++s) {
+                const long long cost = (((long long)base * s + sms - 1) / sms) * ((tiles + s - 1) / s + 4);
+                if (cost < best) { best = cost; splits = s; }
+            }
+        }
+        const auto put = [this](size_t n) {
+            const size_t at = bytes;
+            bytes += (n + 255) / 256 * 256;
+            return at;
+        };
+        bytes = 256;
+        first = put(((size_t)B + 1) * 4);
+        own_ml = put(pieces * 8);
+        own_o = put(pieces * D * 4);
+        const size_t px = (size_t)splits * n_kv * px_rows;
+        px_ml = put(px * 8);
+        px_o = put(px * D * 4);
+    }
+};
+
+template <int D, typename T>
+cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, int n_q, int n_kv, int B, float scale2, char* scratch,
+                            const DecodePlan& pl, cudaStream_t stream) {
+    constexpr bool SPLIT = sizeof(T) == 4;
+    const OwnScratch sc{reinterpret_cast<int*>(scratch), reinterpret_cast<int*>(scratch + pl.first),
+                        reinterpret_cast<float*>(scratch + pl.own_ml), reinterpret_cast<float*>(scratch + pl.own_o)};
+    // The tensor cores take the prefix where its pages are whole swizzle atoms (8 rows) and the copy engine can address
+    // them; else its rows are read like every sequence's own
+    CUtensorMap mk, mv;
+    const bool shared = pl.splits > 0 && kv.kv_shift >= 3 && page_map(&mk, kv.K, D, n_kv, kv) && page_map(&mv, kv.V, D, n_kv, kv);
+    const PrefixScratch px{shared ? pl.splits : 0, pl.px_rows, reinterpret_cast<float*>(scratch + pl.px_ml),
+                           reinterpret_cast<float*>(scratch + pl.px_o)};
+    const int behind = shared ? prefix : 0;
+    cudaError_t st = allow_smem(k_attn_own<D, T>, OwnShape<D>::SMEM);
+    if (st != cudaSuccess) return st;
+    launch_pdl((k_attn_own<D, T>), (unsigned)pl.grid_own, OwnShape<D>::WARPS * 32, OwnShape<D>::SMEM, stream, q, kv, sc, n_q, n_kv, B,
+               behind, scale2, 2);
+    if ((st = launched()) != cudaSuccess) return st;
+    if (shared) {
+        const unsigned grid = (unsigned)((long long)n_kv * pl.row_tiles * pl.splits);
+#define PREFIX(NQ_)                                                                                                       \
+    do {                                                                                                                  \
+        using Ti = typename PrefixShape<D, NQ_, SPLIT>::Ti;                                                               \
+        if ((st = allow_smem(k_attn_prefix<D, NQ_, T>, Ti::SMEM)) != cudaSuccess) return st;                              \
+        launch_pdl((k_attn_prefix<D, NQ_, T>), grid, Ti::WARPS * 32, Ti::SMEM, stream, mk, mv, q, kv, px, n_q, n_kv, B, prefix, scale2, \
+                   pl.row_tiles);                                                                                         \
+    } while (0)
+        if constexpr (D < 256) {
+            if (pl.nq == 2) PREFIX(2); else PREFIX(1);
+        } else {
+            PREFIX(1);
+        }
+#undef PREFIX
+        if ((st = launched()) != cudaSuccess) return st;
+    }
+    launch_pdl((k_attn_join<D, T>), (unsigned)(((long long)B * n_q + 3) / 4), 128, 0, stream, kv, sc, px, out, n_q, n_kv, B, behind);
+    return launched();
+}
+
 template <typename T>
 cudaError_t launch_decode(const T* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,
                           int n_pages, const int* pages, int max_pages, const int* lens, int prefix_len, T* out, int n_q, int n_kv,
                           int D, int B, float scale, void* scratch, size_t scratch_bytes, cudaStream_t stream) {
-    if (!q || !K || !V || !pages || !lens || !out || !good_heads(n_q, n_kv, D) || !good_scale(scale) || B < 1 || n_pages < 1 ||
-        max_pages < 1 || kv_shift < 0 || kv_shift > 30 || kv_stride < (long long)n_kv * D || kv_stride % 8 || kv_bstride % 8 ||
-        kv_bstride < 0 || !al16(q) || !al16(K) || !al16(V) || !al16(out) || (const void*)out == (const void*)q)
+    if (!q || !K || !V || !pages || !lens || !out || !good_heads(n_q, n_kv, D) || !good_scale(scale) || B < 1 ||
+        (long long)B * n_q > (1 << 28) || n_pages < 1 || max_pages < 1 || kv_shift < 0 || kv_shift > 30 ||
+        kv_stride < (long long)n_kv * D || kv_stride % 8 || kv_bstride % 8 || kv_bstride < 0 || !al16(q) || !al16(K) || !al16(V) ||
+        !al16(out) || (const void*)out == (const void*)q)
         return cudaErrorInvalidValue;
     if (prefix_len < 0 || prefix_len % (1 << kv_shift) || prefix_len > ((long long)max_pages << kv_shift)) return cudaErrorInvalidValue;
-    const size_t need = gpu_attn_decode_scratch_bytes(n_q, n_kv, D, B, prefix_len);
-    if (need == 0 || scratch_bytes < need || !scratch || !al16(scratch)) return cudaErrorInvalidValue;
+    const DecodePlan pl(n_q, n_kv, D, B, prefix_len);
+    if (scratch_bytes < pl.bytes || !scratch || !al16(scratch)) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
     const PagedKv kv{reinterpret_cast<const __half*>(K), reinterpret_cast<const __half*>(V), pages, lens, kv_bstride, kv_stride,
                      kv_shift, n_pages, max_pages};
-    const long long grid = ((long long)B * n_q + 3) / 4;
-#define ROWS(D_) launch_pdl((k_attn_decode_rows<D_, T>), (unsigned)grid, 128, 0, stream, q, kv, out, n_q, n_q / n_kv, B, scale * LOG2E)
-    if (D == 64) ROWS(64); else if (D == 128) ROWS(128); else ROWS(256);
-#undef ROWS
-    return launched();
+#define CALL(D_) launch_decode_d<D_, T>(q, kv, prefix_len, out, n_q, n_kv, B, scale * LOG2E, static_cast<char*>(scratch), pl, stream)
+    return D == 64 ? CALL(64) : D == 128 ? CALL(128) : CALL(256);
+#undef CALL
 }
 
 // ---------------------------------------------------------------- pages
@@ -189,8 +286,8 @@ int b200_attn_gave_up(void) {
 }
 
 size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len) {
-    if (!good_heads(n_q, n_kv, head_dim) || B < 1 || prefix_len < 0) return 0;
-    return 256;
+    if (!good_heads(n_q, n_kv, head_dim) || B < 1 || (long long)B * n_q > (1 << 28) || prefix_len < 0) return 0;
+    return DecodePlan(n_q, n_kv, head_dim, B, prefix_len).bytes;
 }
 
 cudaError_t gpu_attn_decode(const float* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,

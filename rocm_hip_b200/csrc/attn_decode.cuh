@@ -1,6 +1,7 @@
 // attn_decode.cuh -- attention of one new token per sequence over a paged FP16 cache. Row t of sequence b is row
 // (t & mask) of page pages[b][t >> kv_shift], a page of the block-major cache being kv_bstride values
-// (kv_row in kv_store.cuh with the page in place of the block).
+// (kv_row in kv_store.cuh with the page in place of the block). Two kernels read the cache, attn_prefix.cuh the rows that
+// the batch shares and attn_own.cuh each sequence's own, a third joins what they found.
 
 #ifndef B200_ATTN_DECODE_CUH
 #define B200_ATTN_DECODE_CUH
@@ -30,31 +31,6 @@ struct PagedKv {
                    ? p * kv_bstride + (long long)(t & ((1 << kv_shift) - 1)) * kv_stride : -1;
     }
 };
-
-template <int D, typename T>
-__global__ void __launch_bounds__(128)
-k_attn_decode_rows(const T* q, PagedKv kv, T* out, int n_q, int G, int B, float scale2) {
-    pdl_entry();
-    constexpr int N = D / 32;
-    const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const int b = (int)(w / n_q), h = (int)(w % n_q), c = (threadIdx.x & 31) * N;
-    if (b >= B) return;
-    float qv[N], kr[N], vr[N];
-    load_vals(q + w * D + c, qv);
-    RowSoftmax<N> st;
-    const int n = kv.len(b);
-    for (int j = 0; j < n; ++j) {
-        const long long r = kv.row(b, j);
-        if (r < 0) continue;
-        load_vals(kv.K + r + h / G * D + c, kr);
-        load_vals(kv.V + r + h / G * D + c, vr);
-        st.key(warp_dot(qv, kr) * scale2, vr);
-    }
-    const float inv = st.l > 0.0f ? 1.0f / st.l : (st.l == 0.0f ? 0.0f : st.l);
-#pragma unroll
-    for (int i = 0; i < N; ++i) st.o[i] *= inv;
-    store_vals(out + w * D + c, st.o);
-}
 
 }  // namespace b200
 

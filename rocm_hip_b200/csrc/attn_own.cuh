@@ -1,0 +1,401 @@
+// attn_own.cuh -- the part of single-token attention that no other sequence shares: each sequence's own cache rows, read
+// once, a warp per key head and stretch of rows. Bound by the cache's bytes (2 D 2 per row and key head); the arithmetic
+// is two small products per 16 rows, which mma.sync does in passing:
+//   S^T [16 rows x 8 heads] = K Q^T          A = K as it lies in the cache, B = the group's queries, in registers
+//   O^T [D x 8 heads]      += V^T P^T        A = V transposed by ldmatrix, B = P by movmatrix
+// Query heads are the narrow side, so a group of up to 8 heads wastes nothing of the wide one (16 query rows as the wide
+// side took twice the products and registers).
+//
+// Queries meet an FP16 cache, so they become fp16 too, without losing anything that counts: a row is scaled by the power
+// of two that takes its largest value to [2^9, 2^10), and fp32 rows are split into q = hi + lo, two fp16 values with 22
+// bits together; weights likewise (P = hi + lo, scaled by 2^P_SHIFT), for bf16 rows hi alone, whose 2^-12 is far below
+// the rounding of the result.
+//
+// Work is dealt out evenly whatever the lengths are: all sequences' row tiles, one after another, are cut into equal
+// shares, one per CTA, so that one long sequence is spread over the device and many short ones share a CTA. Each piece
+// of a sequence leaves (m, l, o) in scratch, and k_attn_join puts the pieces together.
+
+#ifndef B200_ATTN_OWN_CUH
+#define B200_ATTN_OWN_CUH
+
+#include "attn_decode.cuh"
+#include "umma.cuh"
+
+namespace b200 {
+
+constexpr int P_SHIFT = 7;        // weights are held as 2^(s - m + 7): at most 2^15 (m may lag by 2^8), fp16's lower end far away
+constexpr float P_LAG = 8.0f;     // how far a score may exceed m before everything is rescaled
+
+template <int D>
+struct OwnShape {
+    static constexpr int WARPS = D == 256 ? 4 : 8;
+    static constexpr int STAGES = D == 64 ? 6 : 3;
+    static constexpr int STAGE = 2 * 16 * D * 2;                       // 16 rows of K, then 16 of V
+    static constexpr int SMEM = WARPS * STAGES * STAGE;                // 192 KB
+};
+
+// How query heads and rows are spread over a CTA's warps: `units` (key head, up to 8 of its query heads) take a warp each;
+// where that leaves warps over, R row groups of 16 run side by side.
+struct OwnPlan {
+    int gt, units, groups, wh, R, hg;     // tiles of 8 query heads per key head; units; CTA-sized groups of them; units per CTA
+    __host__ __device__ OwnPlan(int n_q, int n_kv, int warps) {
+        const int G = n_q / n_kv;
+        gt = (G + 7) / 8;
+        hg = G < 8 ? G : 8;               // query heads a unit writes at most
+        units = n_kv * gt;
+        groups = (units + warps - 1) / warps;
+        wh = (units + groups - 1) / groups;
+        R = warps / wh;
+    }
+};
+
+// Where the pieces lie in scratch. Slot = CTA + sequence * groups + group: both ascend along the work, so no two pieces
+// share one; a slot holds `warps` pieces of hg heads.
+struct OwnScratch {
+    int* head;        // [0] tiles per CTA
+    int* first;       // [B + 1] tiles before sequence b (of one group)
+    float* ml;        // [slot][warp][hg][2]
+    float* o;         // [slot][warp][hg][D]
+};
+
+__device__ __forceinline__ uint32_t ldsm_addr(const unsigned char* base, int row, int unit, int row_bytes) {
+    return smem_u32(base + row * row_bytes + ((unit ^ (row & 7)) * 16));
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t a, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+__device__ __forceinline__ uint32_t mov_trans(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// 16 bytes, or 16 zeros where `n` is 0
+__device__ __forceinline__ void cp_async16z(uint32_t dst, const void* src, int n) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+
+// The exponent e that takes a row's largest magnitude `top` to [2^9, 2^10) as top * 2^e (0 for a row of zeros or a
+// non-finite one)
+__device__ __forceinline__ int q_exponent(float top) {
+    const int x = (__float_as_int(top) >> 23) & 255;
+    return top > 0.0f && x < 255 ? 9 + 127 - (x ? x : 1) : 0;
+}
+// Rows of its own that sequence b has, and where they begin: behind the shared prefix if it has it whole
+__device__ __forceinline__ int own_rows(const PagedKv& kv, int b, int prefix, int* start) {
+    const int n = kv.len(b);
+    *start = n >= prefix ? prefix : 0;
+    return n - *start;
+}
+
+// QT: type of the queries; SPLIT: two fp16 values per query value and weight
+template <int D, typename QT>
+__global__ void __launch_bounds__(OwnShape<D>::WARPS * 32, 1)
+k_attn_own(const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int prefix, float scale2, int min_tiles) {
+    using Sh = OwnShape<D>;
+    constexpr bool SPLIT = sizeof(QT) == 4;
+    constexpr int W = Sh::WARPS, ST = Sh::STAGES, KS = D / 16, UNITS = D / 8, NT = W * 32;
+    extern __shared__ unsigned char smem_raw[];     // (128-byte swizzle units: 16-byte alignment is enough here)
+    __shared__ int part[NT / 32 + 1], at[4];
+    pdl_entry();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const OwnPlan pl(n_q, n_kv, W);
+    const int G = n_q / n_kv, tile = 16 * pl.R;
+
+    // ---- the shares: every CTA sums the tiles of all sequences, then finds where its own share begins
+    const auto tiles_of = [&](int b) {
+        int s;
+        return b < B ? (own_rows(kv, b, prefix, &s) + tile - 1) / tile : 0;
+    };
+    const auto cta_scan = [&](int v, int* total) {
+        int x = v;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) part[warp] = x;
+        __syncthreads();
+        int base = 0, all = 0;
+        for (int i = 0; i < W; ++i) {
+            base += i < warp ? part[i] : 0;
+            all += part[i];
+        }
+        *total = all;
+        return base + x - v;
+    };
+    int total = 0;
+    for (int b0 = 0; b0 < B; b0 += NT) {
+        int t;
+        const int before = cta_scan(tiles_of(b0 + tid), &t);
+        if (blockIdx.x == 0 && b0 + tid < B) sc.first[b0 + tid] = total + before;
+        total += t;
+    }
+    if (blockIdx.x == 0 && tid == 0) sc.first[B] = total;
+    const long long all = (long long)total * pl.groups;
+    const long long per = max((all + gridDim.x - 1) / gridDim.x, (long long)min_tiles);
+    if (blockIdx.x == 0 && tid == 0) *reinterpret_cast<long long*>(sc.head) = per;
+    long long t0 = blockIdx.x * per;
+    const long long t_end = min(t0 + per, all);
+    if (t0 >= t_end) return;
+    if (tid == 0) at[0] = B;
+    int done = 0;
+    for (int b0 = 0; b0 < B; b0 += NT) {
+        int t;
+        const int n = tiles_of(b0 + tid), before = done + cta_scan(n, &t);
+        if (n > 0 && t0 >= (long long)before * pl.groups && t0 < (long long)(before + n) * pl.groups) {
+            at[0] = b0 + tid;
+            at[1] = (int)(t0 - (long long)before * pl.groups);
+        }
+        done += t;
+    }
+    __syncthreads();
+    int b = at[0], in_seq = at[1];          // the share begins with tile in_seq (counted over the groups) of sequence b
+    if (warp >= pl.wh * pl.R) return;       // (no barrier of the whole CTA from here on)
+
+    unsigned char* ring = smem_raw + warp * ST * Sh::STAGE;
+    const int wu = warp % pl.wh, rg = warp / pl.wh;
+    const int g8 = lane >> 2, t4 = lane & 3;
+    for (; t0 < t_end && b < B; ++b, in_seq = 0) {
+        int start;
+        const int own = own_rows(kv, b, prefix, &start), n_tiles = (own + tile - 1) / tile;
+        while (in_seq < n_tiles * pl.groups && t0 < t_end) {
+            // ---- one piece: tiles [k0, k1) of group `grp` of sequence b
+            const int grp = in_seq / n_tiles, k0 = in_seq - grp * n_tiles;
+            const int k1 = (int)min((long long)n_tiles, k0 + (t_end - t0));
+            in_seq += k1 - k0;
+            t0 += k1 - k0;
+            const int u = grp * pl.wh + wu;
+            if (u >= pl.units) continue;
+            const int kh = u / pl.gt, h0 = u % pl.gt * 8, heads = min(8, G - h0);
+
+            // queries: lane (g8, t4) holds values 16 k + 2 t4 + {0, 1, 8, 9} of head h0 + g8
+            uint32_t qh[KS][2], ql[SPLIT ? KS : 1][2];
+            const QT* qrow = q + ((long long)b * n_q + kh * G + h0 + g8) * D + t4 * 2;
+            float top = 0.0f;
+            if (g8 < heads)
+                for (int i = 0; i < KS * 2; ++i) {
+                    float v[2];
+                    load_vals(qrow + i * 8, v);
+                    top = fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1])));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = q_exponent(top);
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[2] = {0.0f, 0.0f};
+                    if (g8 < heads) load_vals(qrow + i * 16 + p * 8, v);
+                    v[0] = ldexpf(v[0], e);
+                    v[1] = ldexpf(v[1], e);
+                    uint32_t lo;
+                    split16(v[0], v[1], &qh[i][p], &lo);
+                    if constexpr (SPLIT) ql[i][p] = lo;
+                }
+            // score = S c in powers of two; this lane's columns of S^T are heads 2 t4 and 2 t4 + 1
+            const float c_own = ldexpf(scale2, -e);
+            const float c0 = __shfl_sync(0xffffffffu, c_own, t4 * 8), c1 = __shfl_sync(0xffffffffu, c_own, t4 * 8 + 4);
+
+            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, o[KS][4];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+
+            // rows of a tile: lane r (and r + 16) knows where row r lies, -1 if it is not to be seen
+            const auto where = [&](int k) -> long long {
+                const int r = k * tile + rg * 16 + (lane & 15);
+                return k < k1 && r < own ? kv.row(b, start + r) : -1;
+            };
+            unsigned seen[ST];       // which rows of a stage hold a row of the sequence (indexed by unrolled stages only)
+            const auto fetch = [&](int s, long long row) {
+                const uint32_t dst = smem_u32(ring + s * Sh::STAGE);
+#pragma unroll
+                for (int i = 0; i < UNITS / 2; ++i) {
+                    const int x = i * 32 + lane, r = x / UNITS, unit = x % UNITS;
+                    const long long off = __shfl_sync(0xffffffffu, row, r);
+                    const long long src = (off < 0 ? 0 : off) + kh * D + unit * 8;
+                    const uint32_t d = dst + r * (D * 2) + ((unit ^ (r & 7)) * 16);
+                    cp_async16z(d, kv.K + src, off < 0 ? 0 : 16);
+                    cp_async16z(d + 16 * D * 2, kv.V + src, off < 0 ? 0 : 16);
+                }
+                return __ballot_sync(0xffffffffu, row >= 0);
+            };
+            __syncwarp();            // the stages of the piece before have been read
+            long long next = where(k0);
+#pragma unroll
+            for (int s = 0; s < ST - 1; ++s) {
+                const long long row = next;
+                next = where(k0 + s + 1);
+                seen[s] = 0;
+                if (k0 + s < k1) seen[s] = fetch(s, row);
+                cp_async_commit();
+            }
+            for (int k = k0; k < k1; k += ST) {
+#pragma unroll
+                for (int s = 0; s < ST; ++s) {       // stages by constant index
+                    if (k + s < k1) {                // (uniform)
+                        const int f = (s + ST - 1) % ST;
+                        const long long row = next;
+                        next = where(k + s + ST);
+                        seen[f] = 0;
+                        if (k + s + ST - 1 < k1) seen[f] = fetch(f, row);
+                        cp_async_commit();
+                        cp_async_wait<ST - 1>();
+                        __syncwarp();
+                        const unsigned char* Kt = ring + s * Sh::STAGE;
+                        const unsigned char* Vt = Kt + 16 * D * 2;
+                        float st[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) {
+                            uint32_t a[4];
+                            ldsm4(ldsm_addr(Kt, (lane & 7) + (lane >> 3 & 1) * 8, i * 2 + (lane >> 4), D * 2), a);
+                            if constexpr (SPLIT) mma16(st, a, ql[i][0], ql[i][1]);
+                            mma16(st, a, qh[i][0], qh[i][1]);
+                        }
+                        const bool s0 = seen[s] >> g8 & 1, s1 = seen[s] >> (g8 + 8) & 1;
+                        const float x0 = s0 ? st[0] * c0 : -INFINITY, x1 = s0 ? st[1] * c1 : -INFINITY;
+                        const float x2 = s1 ? st[2] * c0 : -INFINITY, x3 = s1 ? st[3] * c1 : -INFINITY;
+                        if (__any_sync(0xffffffffu, fmaxf(x0, x2) > m0 + P_LAG || fmaxf(x1, x3) > m1 + P_LAG)) {
+                            float n0 = fmaxf(m0, fmaxf(x0, x2)), n1 = fmaxf(m1, fmaxf(x1, x3));
+#pragma unroll
+                            for (int off = 4; off < 32; off <<= 1) {
+                                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, off));
+                                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, off));
+                            }
+                            const float f0 = n0 == -INFINITY ? 1.0f : ex2(m0 - n0), f1 = n1 == -INFINITY ? 1.0f : ex2(m1 - n1);
+                            m0 = n0;
+                            m1 = n1;
+                            l0 *= f0;
+                            l1 *= f1;
+#pragma unroll
+                            for (int i = 0; i < KS; ++i) {
+                                o[i][0] *= f0;
+                                o[i][1] *= f1;
+                                o[i][2] *= f0;
+                                o[i][3] *= f1;
+                            }
+                        }
+                        const float e0 = m0 == -INFINITY ? 0.0f : P_SHIFT - m0, e1 = m1 == -INFINITY ? 0.0f : P_SHIFT - m1;
+                        const float p0 = ex2(x0 + e0), p1 = ex2(x1 + e1), p2 = ex2(x2 + e0), p3 = ex2(x3 + e1);
+                        l0 += p0 + p2;
+                        l1 += p1 + p3;
+                        uint32_t h01, h23, w01, w23;
+                        split16(p0, p1, &h01, &w01);
+                        split16(p2, p3, &h23, &w23);
+                        const uint32_t b0 = mov_trans(h01), b1 = mov_trans(h23);
+                        uint32_t d0 = 0, d1 = 0;
+                        if constexpr (SPLIT) {
+                            d0 = mov_trans(w01);
+                            d1 = mov_trans(w23);
+                        }
+#pragma unroll
+                        for (int i = 0; i < KS; ++i) {
+                            uint32_t a[4];
+                            ldsm4t(ldsm_addr(Vt, (lane & 7) + (lane >> 4) * 8, i * 2 + (lane >> 3 & 1), D * 2), a);
+                            mma16(o[i], a, b0, b1);
+                            if constexpr (SPLIT) mma16(o[i], a, d0, d1);
+                        }
+                        __syncwarp();
+                    }
+                }
+            }
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) {
+                l0 += __shfl_xor_sync(0xffffffffu, l0, off);
+                l1 += __shfl_xor_sync(0xffffffffu, l1, off);
+            }
+            const long long piece = ((long long)(blockIdx.x + (long long)b * pl.groups + grp) * W + warp) * pl.hg;
+            if (g8 == 0) {
+                if (2 * t4 < heads) { sc.ml[(piece + 2 * t4) * 2] = m0; sc.ml[(piece + 2 * t4) * 2 + 1] = l0; }
+                if (2 * t4 + 1 < heads) { sc.ml[(piece + 2 * t4 + 1) * 2] = m1; sc.ml[(piece + 2 * t4 + 1) * 2 + 1] = l1; }
+            }
+            float* po = sc.o + piece * D;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const int d = i * 16 + g8;
+                if (2 * t4 < heads) { po[2 * t4 * D + d] = o[i][0]; po[2 * t4 * D + d + 8] = o[i][2]; }
+                if (2 * t4 + 1 < heads) { po[(2 * t4 + 1) * D + d] = o[i][1]; po[(2 * t4 + 1) * D + d + 8] = o[i][3]; }
+            }
+        }
+    }
+    cp_async_wait_all();
+}
+
+// The pieces the prefix kernel leaves: [split][key head][row b G + g]
+struct PrefixScratch {
+    int splits;       // 0: there is none
+    long long rows;   // B G rounded up to whole tiles
+    float* ml;        // [split][n_kv][rows][2]
+    float* o;         // [split][n_kv][rows][D]
+};
+
+// out[b, h] = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i over the pieces i of the row, in the order of the rows they
+// cover; a row without pieces, or with none that saw a key, is zero. A warp per row.
+template <int D, typename QT>
+__global__ void __launch_bounds__(128)
+k_attn_join(PagedKv kv, OwnScratch sc, PrefixScratch px, QT* out, int n_q, int n_kv, int B, int prefix) {
+    pdl_entry();
+    constexpr int N = D / 32, W = OwnShape<D>::WARPS;
+    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (row >= (long long)B * n_q) return;
+    const int b = (int)(row / n_q), h = (int)(row % n_q), G = n_q / n_kv, kh = h / G, g = h % G;
+    const OwnPlan pl(n_q, n_kv, W);
+    const int u = kh * pl.gt + g / 8, grp = u / pl.wh, wu = u % pl.wh;
+    const long long per = *reinterpret_cast<const long long*>(sc.head);
+    const int n_tiles = sc.first[b + 1] - sc.first[b];
+    const long long t0 = (long long)sc.first[b] * pl.groups + (long long)grp * n_tiles;
+    const int c0 = n_tiles ? (int)(t0 / per) : 0, n_own = n_tiles ? ((int)((t0 + n_tiles - 1) / per) - c0 + 1) * pl.R : 0;
+    const int n_px = kv.len(b) >= prefix ? px.splits : 0, n = n_px + n_own;
+    // piece i of the row -> its (m, l) and o
+    const auto piece = [&](int i, const float** o) -> const float* {
+        if (i < n_px) {
+            const long long at = ((long long)i * n_kv + kh) * px.rows + (long long)b * G + g;
+            *o = px.o + at * D;
+            return px.ml + at * 2;
+        }
+        i -= n_px;
+        const long long slot = c0 + i / pl.R + (long long)b * pl.groups + grp;
+        const long long at = (slot * W + wu + i % pl.R * pl.wh) * pl.hg + g % 8;
+        *o = sc.o + at * D;
+        return sc.ml + at * 2;
+    };
+    float M = -INFINITY;
+    for (int i = lane; i < n; i += 32) {
+        const float* o;
+        M = fmaxf(M, piece(i, &o)[0]);
+    }
+#pragma unroll
+    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+    float l = 0.0f, acc[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = 0.0f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+        const float* o;
+        const float* ml = piece(i, &o);
+        const float mi = ml[0], f = mi == -INFINITY ? 0.0f : ex2(mi - M);
+        float v[N];
+        load_vals(o + lane * N, v);
+        l += f * ml[1];
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] += f * v[e];
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] *= inv;
+    store_vals(out + row * D + lane * N, acc);
+}
+
+}  // namespace b200
+
+#endif  // B200_ATTN_OWN_CUH

@@ -1,0 +1,177 @@
+// attn_prefix.cuh -- the part of single-token attention that the whole batch shares: the prefix's rows, read once. The
+// queries of all sequences that read one key head are the rows of a product, B G of them, and the kernel is the tile
+// kernel of the prompts without its mask: CTA = (key head, 128 or 256 query rows, a stretch of the prefix), K and V tiles
+// by TMA straight out of the cache's pages. Each CTA leaves (m, l, o) of its stretch for k_attn_join.
+//
+// Queries become fp16 as in attn_own.cuh: scaled by a power of two per row, fp32 ones as hi + lo.
+
+#ifndef B200_ATTN_PREFIX_CUH
+#define B200_ATTN_PREFIX_CUH
+
+#include "attn_own.cuh"
+#include "attn_tiles.cuh"
+
+namespace b200 {
+
+template <int D, int NQ, bool SPLIT>
+struct PrefixShape {
+    // fp32 queries of 256-wide heads take 128 KB: stages of 64 columns, so that six of them fit beside
+    static constexpr int SC = D == 64 || (D == 256 && SPLIT) ? 64 : 128;
+    static constexpr int Q_BYTES = NQ * TILE_ROWS * D * 2 * (SPLIT ? 2 : 1);
+    static constexpr int FIT = (230400 - 1024 - Q_BYTES) / (TILE_ROWS * SC * 2);
+    static constexpr int ST = FIT < 8 ? FIT : 8;
+    using Ti = Tiles<D, NQ, SC, ST, SPLIT, __half>;
+};
+
+template <int D, int NQ, typename QT>
+__global__ void __launch_bounds__(PrefixShape<D, NQ, sizeof(QT) == 4>::Ti::WARPS * 32, 1)
+k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const QT* q, PagedKv kv, PrefixScratch px,
+              int n_q, int n_kv, int B, int prefix, float scale2, int row_tiles) {
+    constexpr bool SPLIT = sizeof(QT) == 4;
+    using Ti = typename PrefixShape<D, NQ, SPLIT>::Ti;
+    constexpr int SC = PrefixShape<D, NQ, SPLIT>::SC, N = D / 32;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ TileBars bars;
+    unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    unsigned char* ring = smem + Ti::Q_BYTES;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = n_q / n_kv;
+    if (warp == NQ * 4 + 1 && lane == 0) {
+        tma_prefetch(&mk);
+        tma_prefetch(&mv);
+    }
+    Ti::setup(bars, NQ * 4);
+    // No wait for the kernel before this one (k_attn_own) here: it began after its own predecessors were done, it writes
+    // nothing that is read here, and this kernel starts only once all of its CTAs have begun. The wait at the end makes
+    // this kernel's completion stand for both.
+
+    const int kh = blockIdx.x % n_kv, rt = blockIdx.x / n_kv % row_tiles, split = blockIdx.x / n_kv / row_tiles;
+    const int tiles = (prefix + TILE_ROWS - 1) / TILE_ROWS;
+    const int j0 = (int)((long long)tiles * split / px.splits), j1 = (int)((long long)tiles * (split + 1) / px.splits);
+    const int M = B * G, r0 = rt * NQ * TILE_ROWS;
+    // the prefix's pages: the list of the first sequence that has all of it
+    const int* pages = nullptr;
+    for (int b0 = 0; b0 < B && !pages; b0 += 32) {
+        const unsigned has = __ballot_sync(0xffffffffu, b0 + lane < B && kv.len(b0 + lane) >= prefix);
+        if (has) pages = kv.pages + (long long)(b0 + __ffs(has) - 1) * kv.max_pages;
+    }
+    if (pages) {   // else nobody reads what this kernel would write
+    int n[2] = {j1 - j0, NQ == 2 && r0 + TILE_ROWS < M ? j1 - j0 : 0};
+    const int n_all = n[0];
+
+    if (warp == NQ * 4 + 1) {
+        Ti::few_registers();
+        if (lane == 0) {
+            const int in_page = 1 << kv.kv_shift, box = min(in_page, TILE_ROWS);
+            typename Ti::Ring r{bars, ring};
+            const auto put = [&](const CUtensorMap* map, int j) {
+                r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
+                    for (int a = 0; a < TILE_ROWS; a += box) {
+                        // rows behind the prefix and pages outside the cache: page -1, which the copy fills with zeros
+                        const int t = (j0 + j) * TILE_ROWS + a;
+                        int page = t < prefix ? pages[t >> kv.kv_shift] : -1;
+                        if ((unsigned)page >= (unsigned)kv.n_pages) page = -1;
+                        for (int c = 0; c < SC / CHUNK; ++c)
+                            tma_4d(dst + c * CHUNK_BYTES + a * 128, map, p * SC + c * CHUNK, kh, t & (in_page - 1), page, bar);
+                    }
+                });
+            };
+            put(&mk, 0);
+            for (int j = 0; j < n_all; ++j) {
+                if (j + 1 < n_all) put(&mk, j + 1);
+                put(&mv, j);
+            }
+        }
+    } else if (warp == NQ * 4) {
+        Ti::few_registers();
+        if (lane == 0) Ti::products(bars, smem, ring, n);
+    } else if (warp < NQ * 4) {
+        Ti::many_registers();
+        const int i = warp >> 2, mine = r0 + warp * 32;     // this warp's 32 query rows
+        // ---- queries to shared memory, a row of D values by the whole warp: K-major, 128-byte swizzle
+        float c_row = 0.0f;
+#pragma unroll 4
+        for (int rr = 0; rr < 32; ++rr) {
+            const int r = mine + rr;
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) v[e] = 0.0f;
+            if (r < M) load_vals(q + ((long long)(r / G) * n_q + kh * G + r % G) * D + lane * N, v);
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; ++e) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const int x = q_exponent(top);
+            if (lane == rr) c_row = ldexpf(scale2, -x);
+            const int col = lane * N, in_tile = (warp & 3) * 32 + rr;
+            unsigned char* at = smem + i * Ti::QTILE * (SPLIT ? 2 : 1) + col / CHUNK * CHUNK_BYTES + in_tile * 128 +
+                                (((col % CHUNK / 8) ^ (in_tile & 7)) * 16) + col % 8 * 2;
+#pragma unroll
+            for (int e = 0; e < N; e += 2) {
+                uint32_t hi, lo;
+                split16(ldexpf(v[e], x), ldexpf(v[e + 1], x), &hi, &lo);
+                *reinterpret_cast<uint32_t*>(at + e * 2) = hi;
+                if constexpr (SPLIT) *reinterpret_cast<uint32_t*>(at + Ti::QTILE + e * 2) = lo;
+            }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.q_full);
+
+        float m = -INFINITY, l = 0.0f;
+        const int tiles_i = i ? n[1] : n[0];
+        // four neighbouring rows of a tile are in one page: lane k speaks for keys 4 k .. 4 k + 3
+        const auto look = [&](int j) {
+            const int t = (j0 + j) * TILE_ROWS + lane * 4;
+            return j < tiles_i && t < prefix && (unsigned)pages[t >> kv.kv_shift] < (unsigned)kv.n_pages;
+        };
+        bool next = look(0);
+        for (int j = 0; j < tiles_i; ++j) {
+            const unsigned seen = __ballot_sync(0xffffffffu, next);
+            next = look(j + 1);
+            uint32_t x[128];
+            if (!Ti::scores(bars, i, j, x)) break;
+            if (seen != 0xffffffffu)
+#pragma unroll
+                for (int e = 0; e < 128; ++e)
+                    if (!(seen >> (e / 4) & 1)) x[e] = 0xff800000u;
+            if (!Ti::weights(bars, i, j, x, c_row, m, l)) break;
+        }
+        if (tiles_i > 0 && wait_or_die(&bars.o_full[i], 0, &bars.dead)) {
+            tc_fence_after();
+            const uint32_t o_addr = bars.tmem + 256 + i * D + ((uint32_t)(threadIdx.x & 96) << 16);
+            const long long at = ((long long)split * n_kv + kh) * px.rows + mine;
+            px.ml[(at + lane) * 2] = m == -INFINITY ? -INFINITY : m * c_row;
+            px.ml[(at + lane) * 2 + 1] = l;
+            // through this warp's part of the query tile (32 rows of at least 128 bytes), 32 columns at a time
+            float* buf = reinterpret_cast<float*>(smem + (i * TILE_ROWS + (warp & 3) * 32) * (D * 2 * (SPLIT ? 2 : 1)));
+            static_assert(32 * 32 * 4 <= 32 * D * 2, "32 rows of 32 floats fit the warp's part");
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                tmem_ld32(o_addr + c, o);
+                tmem_ld_wait();
+                tmem_pin(o);
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<uint4*>(buf + lane * 32 + ((e / 4 ^ (lane & 7)) * 4)) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int rr = e * 4 + (lane >> 3), u = lane & 7;
+                    *reinterpret_cast<uint4*>(px.o + (at + rr) * D + c + u * 4) =
+                        *reinterpret_cast<const uint4*>(buf + rr * 32 + ((u ^ (rr & 7)) * 4));
+                }
+                __syncwarp();
+            }
+        }
+    } else {
+        Ti::few_registers();
+    }
+    }
+    Ti::teardown(bars);
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+}  // namespace b200
+
+#endif  // B200_ATTN_PREFIX_CUH

@@ -118,6 +118,14 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     else return pack_f16(lo, hi);
 }
 
+// v as fp16 hi (+ lo)
+__device__ __forceinline__ void split16(float a, float b, uint32_t* hi, uint32_t* lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    *hi = *reinterpret_cast<const uint32_t*>(&h);
+    *lo = pack_f16(a - f.x, b - f.y);
+}
+
 }  // namespace b200
 
 #endif  // B200_UMMA_CUH
