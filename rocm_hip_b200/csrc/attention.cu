@@ -110,13 +110,13 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
 
 // ---------------------------------------------------------------- single tokens
 
-// The pages of one half (K or V) of a layer, fetched as boxes of up to 128 rows x 64 values of one head
-bool page_map(CUtensorMap* m, const __half* p, int D, int heads, const PagedKv& kv) {
+// The pages of one half (K or V) of a layer, fetched as boxes of up to `rows` rows x 64 values of one head
+bool page_map(CUtensorMap* m, const __half* p, int D, int heads, const PagedKv& kv, int rows) {
     const int in_page = 1 << kv.kv_shift;
     const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)in_page, (cuuint64_t)kv.n_pages};
     const cuuint64_t strides[3] = {(cuuint64_t)D * 2, (cuuint64_t)kv.kv_stride * 2,
                                    (cuuint64_t)(kv.n_pages > 1 ? kv.kv_bstride : kv.kv_stride) * 2};
-    const cuuint32_t box[4] = {CHUNK, 1, (cuuint32_t)(in_page < TILE_ROWS ? in_page : TILE_ROWS), 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {CHUNK, 1, (cuuint32_t)(in_page < rows ? in_page : rows), 1}, step[4] = {1, 1, 1, 1};
     const auto fn = encode_fn();
     return fn && fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<__half*>(p), dims, strides, box, step,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -173,17 +173,23 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
     constexpr bool SPLIT = sizeof(T) == 4;
     const OwnScratch sc{reinterpret_cast<int*>(scratch), reinterpret_cast<int*>(scratch + pl.first),
                         reinterpret_cast<float*>(scratch + pl.own_ml), reinterpret_cast<float*>(scratch + pl.own_o)};
-    // The tensor cores take the prefix where its pages are whole swizzle atoms (8 rows) and the copy engine can address
-    // them; else its rows are read like every sequence's own
-    CUtensorMap mk, mv;
-    const bool shared = pl.splits > 0 && kv.kv_shift >= 3 && page_map(&mk, kv.K, D, n_kv, kv) && page_map(&mv, kv.V, D, n_kv, kv);
+    // The copy engine takes the cache apart where pages are whole swizzle atoms (8 rows) and a tensor map can describe it;
+    // else a prefix is read like every sequence's own rows, and those by the threads
+    CUtensorMap mk, mv, ok, ov;
+    const bool box = kv.kv_shift >= 3 && page_map(&ok, kv.K, D, n_kv, kv, 16) && page_map(&ov, kv.V, D, n_kv, kv, 16);
+    const bool shared = pl.splits > 0 && box && page_map(&mk, kv.K, D, n_kv, kv, TILE_ROWS) && page_map(&mv, kv.V, D, n_kv, kv, TILE_ROWS);
     const PrefixScratch px{shared ? pl.splits : 0, pl.px_rows, reinterpret_cast<float*>(scratch + pl.px_ml),
                            reinterpret_cast<float*>(scratch + pl.px_o)};
     const int behind = shared ? prefix : 0;
-    cudaError_t st = allow_smem(k_attn_own<D, T>, OwnShape<D>::SMEM);
-    if (st != cudaSuccess) return st;
-    launch_pdl((k_attn_own<D, T>), (unsigned)pl.grid_own, OwnShape<D>::WARPS * 32, OwnShape<D>::SMEM, stream, q, kv, sc, n_q, n_kv, B,
-               behind, scale2, 2);
+    cudaError_t st;
+#define OWN(BOX_)                                                                                                            \
+    do {                                                                                                                     \
+        if ((st = allow_smem(k_attn_own<D, T, BOX_>, OwnShape<D>::SMEM)) != cudaSuccess) return st;                          \
+        launch_pdl((k_attn_own<D, T, BOX_>), (unsigned)pl.grid_own, OwnShape<D>::WARPS * 32, OwnShape<D>::SMEM, stream, ok, ov, q, kv, \
+                   sc, n_q, n_kv, B, behind, scale2, 2);                                                                     \
+    } while (0)
+    if (box) OWN(true); else OWN(false);
+#undef OWN
     if ((st = launched()) != cudaSuccess) return st;
     if (shared) {
         const unsigned grid = (unsigned)((long long)n_kv * pl.row_tiles * pl.splits);

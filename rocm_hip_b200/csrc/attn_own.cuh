@@ -19,7 +19,7 @@
 #define B200_ATTN_OWN_CUH
 
 #include "attn_decode.cuh"
-#include "umma.cuh"
+#include "attn_tiles.cuh"
 
 namespace b200 {
 
@@ -31,7 +31,7 @@ struct OwnShape {
     static constexpr int WARPS = D == 256 ? 4 : 8;
     static constexpr int STAGES = D == 64 ? 6 : 3;
     static constexpr int STAGE = 2 * 16 * D * 2;                       // 16 rows of K, then 16 of V
-    static constexpr int SMEM = WARPS * STAGES * STAGE;                // 192 KB
+    static constexpr int SMEM = 1024 + WARPS * STAGES * STAGE;         // 193 KB
 };
 
 // How query heads and rows are spread over a CTA's warps: `units` (key head, up to 8 of its query heads) take a warp each;
@@ -58,9 +58,9 @@ struct OwnScratch {
     float* o;         // [slot][warp][hg][D]
 };
 
-__device__ __forceinline__ uint32_t ldsm_addr(const unsigned char* base, int row, int unit, int row_bytes) {
-    return smem_u32(base + row * row_bytes + ((unit ^ (row & 7)) * 16));
-}
+// A tile of 16 rows in shared memory: chunks of 64 values, [16 rows][128 bytes], 16-byte units swizzled as the copy engine
+// does (unit ^ row mod 8), so that ldmatrix meets no bank twice
+__device__ __forceinline__ uint32_t own_at(int row, int unit) { return unit / 8 * 2048 + row * 128 + ((unit & 7) ^ (row & 7)) * 16; }
 __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
 }
@@ -95,17 +95,28 @@ __device__ __forceinline__ int own_rows(const PagedKv& kv, int b, int prefix, in
     return n - *start;
 }
 
-// QT: type of the queries; SPLIT: two fp16 values per query value and weight
-template <int D, typename QT>
+// QT: type of the queries (fp32: two fp16 values per query value and weight). BOX: tiles come by the copy engine, in boxes
+// of 8 or 16 rows of a page, at four instructions a tile; a thread's own 16-byte copies, the other way, cost a third of
+// all instructions (64 sequences of 1 .. 2,048 rows, 8 heads of 128: 62 us) and serve pages of fewer rows and caches that a
+// tensor map cannot describe.
+template <int D, typename QT, bool BOX>
 __global__ void __launch_bounds__(OwnShape<D>::WARPS * 32, 1)
-k_attn_own(const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int prefix, float scale2, int min_tiles) {
+k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int prefix, float scale2, int min_tiles) {
     using Sh = OwnShape<D>;
     constexpr bool SPLIT = sizeof(QT) == 4;
     constexpr int W = Sh::WARPS, ST = Sh::STAGES, KS = D / 16, UNITS = D / 8, NT = W * 32;
-    extern __shared__ unsigned char smem_raw[];     // (128-byte swizzle units: 16-byte alignment is enough here)
+    extern __shared__ unsigned char smem_raw[];
     __shared__ int part[NT / 32 + 1], at[4];
-    pdl_entry();
+    __shared__ unsigned long long full[W][ST];
+    unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (BOX && lane == 0) {
+        for (int i = 0; i < ST; ++i) mbar_init(&full[warp][i], 1);
+        mbar_fence_init();
+        tma_prefetch(&mk);
+        tma_prefetch(&mv);
+    }
+    pdl_entry();
     const OwnPlan pl(n_q, n_kv, W);
     const int G = n_q / n_kv, tile = 16 * pl.R;
 
@@ -161,7 +172,9 @@ k_attn_own(const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int
     int b = at[0], in_seq = at[1];          // the share begins with tile in_seq (counted over the groups) of sequence b
     if (warp >= pl.wh * pl.R) return;       // (no barrier of the whole CTA from here on)
 
-    unsigned char* ring = smem_raw + warp * ST * Sh::STAGE;
+    unsigned char* ring = smem + warp * ST * Sh::STAGE;
+    unsigned phases = 0;                    // bit s: the parity stage s completes next
+    bool alive = true;
     const int wu = warp % pl.wh, rg = warp / pl.wh;
     const int g8 = lane >> 2, t4 = lane & 3;
     for (; t0 < t_end && b < B; ++b, in_seq = 0) {
@@ -210,57 +223,103 @@ k_attn_own(const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int
 #pragma unroll
             for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
-            // rows of a tile: lane r (and r + 16) knows where row r lies, -1 if it is not to be seen
+            // Where tile k begins. BOX: lane 0 issues the copies, so every lane holds the same first page; the second one of
+            // a tile over two 8-row pages is its neighbour in the list. Else lane r holds where row r lies. -1: not there.
             const auto where = [&](int k) -> long long {
-                const int r = k * tile + rg * 16 + (lane & 15);
-                return k < k1 && r < own ? kv.row(b, start + r) : -1;
+                const int r = k * tile + rg * 16 + (BOX ? 0 : lane & 15);
+                if (k >= k1 || r >= own) return -1;
+                if constexpr (!BOX) return kv.row(b, start + r);
+                const int* list = kv.pages + (long long)b * kv.max_pages + ((start + r) >> kv.kv_shift);
+                const unsigned p0 = list[0], n = kv.n_pages;
+                unsigned p1 = n;
+                if (kv.kv_shift == 3 && r + 8 < own) p1 = list[1];
+                return ((long long)(p1 < n ? p1 : -1) << 32) | (unsigned)(p0 < n ? p0 : -1);
             };
             unsigned seen[ST];       // which rows of a stage hold a row of the sequence (indexed by unrolled stages only)
-            const auto fetch = [&](int s, long long row) {
-                const uint32_t dst = smem_u32(ring + s * Sh::STAGE);
+            const auto fetch = [&](int s, int k, long long at) -> unsigned {
+                if constexpr (BOX) {
+                    const int p0 = (int)at, p1 = (int)(at >> 32), r = k * tile + rg * 16, t = start + r;
+                    if (lane == 0) {
+                        fence_async_smem();      // the rows that a tail blanked in this stage
+                        unsigned char* dst = ring + s * Sh::STAGE;
+                        mbar_expect(&full[warp][s], Sh::STAGE);
+                        const int in_page = t & ((1 << kv.kv_shift) - 1);
 #pragma unroll
-                for (int i = 0; i < UNITS / 2; ++i) {
-                    const int x = i * 32 + lane, r = x / UNITS, unit = x % UNITS;
-                    const long long off = __shfl_sync(0xffffffffu, row, r);
-                    const long long src = (off < 0 ? 0 : off) + kh * D + unit * 8;
-                    const uint32_t d = dst + r * (D * 2) + ((unit ^ (r & 7)) * 16);
-                    cp_async16z(d, kv.K + src, off < 0 ? 0 : 16);
-                    cp_async16z(d + 16 * D * 2, kv.V + src, off < 0 ? 0 : 16);
+                        for (int c = 0; c < D / CHUNK; ++c) {
+                            tma_4d(dst + c * 2048, &mk, c * CHUNK, kh, in_page, p0, &full[warp][s]);
+                            tma_4d(dst + 16 * D * 2 + c * 2048, &mv, c * CHUNK, kh, in_page, p0, &full[warp][s]);
+                            if (kv.kv_shift == 3) {
+                                tma_4d(dst + c * 2048 + 1024, &mk, c * CHUNK, kh, 0, p1, &full[warp][s]);
+                                tma_4d(dst + 16 * D * 2 + c * 2048 + 1024, &mv, c * CHUNK, kh, 0, p1, &full[warp][s]);
+                            }
+                        }
+                    }
+                    const unsigned rows = own - r >= 16 ? 0xffffu : own - r > 0 ? (1u << (own - r)) - 1 : 0;
+                    const unsigned pages = kv.kv_shift == 3 ? (p0 >= 0 ? 0xffu : 0) | (p1 >= 0 ? 0xff00u : 0) : p0 >= 0 ? 0xffffu : 0;
+                    return rows & pages;
+                } else {
+                    const uint32_t dst = smem_u32(ring + s * Sh::STAGE);
+#pragma unroll
+                    for (int i = 0; i < UNITS / 2; ++i) {
+                        const int x = i * 32 + lane, r = x / UNITS, unit = x % UNITS;
+                        const long long off = __shfl_sync(0xffffffffu, at, r);
+                        const long long src = (off < 0 ? 0 : off) + kh * D + unit * 8;
+                        const uint32_t d = dst + own_at(r, unit);
+                        cp_async16z(d, kv.K + src, off < 0 ? 0 : 16);
+                        cp_async16z(d + 16 * D * 2, kv.V + src, off < 0 ? 0 : 16);
+                    }
+                    return __ballot_sync(0xffffffffu, at >= 0) & 0xffffu;
                 }
-                return __ballot_sync(0xffffffffu, row >= 0);
             };
             __syncwarp();            // the stages of the piece before have been read
             long long next = where(k0);
 #pragma unroll
             for (int s = 0; s < ST - 1; ++s) {
-                const long long row = next;
+                const long long at = next;
                 next = where(k0 + s + 1);
                 seen[s] = 0;
-                if (k0 + s < k1) seen[s] = fetch(s, row);
-                cp_async_commit();
+                if (k0 + s < k1) seen[s] = fetch(s, k0 + s, at);
+                if (!BOX) cp_async_commit();
             }
             for (int k = k0; k < k1; k += ST) {
 #pragma unroll
                 for (int s = 0; s < ST; ++s) {       // stages by constant index
                     if (k + s < k1) {                // (uniform)
                         const int f = (s + ST - 1) % ST;
-                        const long long row = next;
+                        const long long at = next;
                         next = where(k + s + ST);
                         seen[f] = 0;
-                        if (k + s + ST - 1 < k1) seen[f] = fetch(f, row);
-                        cp_async_commit();
-                        cp_async_wait<ST - 1>();
-                        __syncwarp();
-                        const unsigned char* Kt = ring + s * Sh::STAGE;
-                        const unsigned char* Vt = Kt + 16 * D * 2;
-                        float st[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                        for (int i = 0; i < KS; ++i) {
-                            uint32_t a[4];
-                            ldsm4(ldsm_addr(Kt, (lane & 7) + (lane >> 3 & 1) * 8, i * 2 + (lane >> 4), D * 2), a);
-                            if constexpr (SPLIT) mma16(st, a, ql[i][0], ql[i][1]);
-                            mma16(st, a, qh[i][0], qh[i][1]);
+                        if (k + s + ST - 1 < k1) seen[f] = fetch(f, k + s + ST - 1, at);
+                        unsigned char* Kt = ring + s * Sh::STAGE;
+                        unsigned char* Vt = Kt + 16 * D * 2;
+                        if constexpr (BOX) {
+                            if (alive) alive = mbar_wait(&full[warp][s], phases >> s & 1);
+                            phases ^= 1u << s;
+                            if (seen[s] != 0xffffu) {   // a weight of 0 needs a finite v: what lies behind the sequence is blanked
+                                for (int e = lane; e < 16 * UNITS; e += 32)
+                                    if (!(seen[s] >> (e / UNITS) & 1)) *reinterpret_cast<uint4*>(Vt + own_at(e / UNITS, e % UNITS)) = make_uint4(0, 0, 0, 0);
+                            }
+                        } else {
+                            cp_async_commit();
+                            cp_async_wait<ST - 1>();
                         }
+                        __syncwarp();
+                        // two chains of products, so that one's latency hides the other's
+                        float st[4] = {0.0f, 0.0f, 0.0f, 0.0f}, su[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < KS; i += 2) {
+                            uint32_t a[4], c[4];
+                            ldsm4(smem_u32(Kt) + own_at((lane & 7) + (lane >> 3 & 1) * 8, i * 2 + (lane >> 4)), a);
+                            ldsm4(smem_u32(Kt) + own_at((lane & 7) + (lane >> 3 & 1) * 8, i * 2 + 2 + (lane >> 4)), c);
+                            if constexpr (SPLIT) {
+                                mma16(st, a, ql[i][0], ql[i][1]);
+                                mma16(su, c, ql[i + 1][0], ql[i + 1][1]);
+                            }
+                            mma16(st, a, qh[i][0], qh[i][1]);
+                            mma16(su, c, qh[i + 1][0], qh[i + 1][1]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) st[i] += su[i];
                         const bool s0 = seen[s] >> g8 & 1, s1 = seen[s] >> (g8 + 8) & 1;
                         const float x0 = s0 ? st[0] * c0 : -INFINITY, x1 = s0 ? st[1] * c1 : -INFINITY;
                         const float x2 = s1 ? st[2] * c0 : -INFINITY, x3 = s1 ? st[3] * c1 : -INFINITY;
@@ -300,7 +359,7 @@ k_attn_own(const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int
 #pragma unroll
                         for (int i = 0; i < KS; ++i) {
                             uint32_t a[4];
-                            ldsm4t(ldsm_addr(Vt, (lane & 7) + (lane >> 4) * 8, i * 2 + (lane >> 3 & 1), D * 2), a);
+                            ldsm4t(smem_u32(Vt) + own_at((lane & 7) + (lane >> 4) * 8, i * 2 + (lane >> 3 & 1)), a);
                             mma16(o[i], a, b0, b1);
                             if constexpr (SPLIT) mma16(o[i], a, d0, d1);
                         }
@@ -327,7 +386,8 @@ k_attn_own(const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int
             }
         }
     }
-    cp_async_wait_all();
+    if (!BOX) cp_async_wait_all();
+    if (!alive && lane == 0) atomicAdd(&attn_gave_up, 1);
 }
 
 // The pieces the prefix kernel leaves: [split][key head][row b G + g]
@@ -369,26 +429,45 @@ k_attn_join(PagedKv kv, OwnScratch sc, PrefixScratch px, QT* out, int n_q, int n
         *o = sc.o + at * D;
         return sc.ml + at * 2;
     };
-    float M = -INFINITY;
-    for (int i = lane; i < n; i += 32) {
-        const float* o;
-        M = fmaxf(M, piece(i, &o)[0]);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-    float l = 0.0f, acc[N];
+    // lane i takes piece i of every 32: its m, l and where its o lies
+    float M = -INFINITY, l = 0.0f, acc[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] = 0.0f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-        const float* o;
-        const float* ml = piece(i, &o);
-        const float mi = ml[0], f = mi == -INFINITY ? 0.0f : ex2(mi - M);
-        float v[N];
-        load_vals(o + lane * N, v);
-        l += f * ml[1];
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        const float* mine = nullptr;
+        float mi = -INFINITY, li = 0.0f;
+        if (i0 + lane < n) {
+            const float* ml = piece(i0 + lane, &mine);
+            mi = ml[0];
+            li = ml[1];
+        }
+        float top = fmaxf(M, mi);
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += f * v[e];
+        for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+        const float old = M == -INFINITY ? 0.0f : ex2(M - top), f = mi == -INFINITY ? 0.0f : ex2(mi - top);
+        float sum = f * li;
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        l = l * old + sum;
+        M = top;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[e] *= old;
+        const int count = min(32, n - i0);
+        for (int i = 0; i < count; i += 8) {    // eight rows in flight
+            float v[8][N];
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)mine, i + t));
+                if (i + t < count) load_vals(o + lane * N, v[t]);
+            }
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const float ft = __shfl_sync(0xffffffffu, f, i + t);
+                if (i + t < count)
+#pragma unroll
+                    for (int e = 0; e < N; ++e) acc[e] += ft * v[t][e];
+            }
+        }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll

@@ -60,26 +60,34 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
 
     if (warp == NQ * 4 + 1) {
         Ti::few_registers();
-        if (lane == 0) {
-            const int in_page = 1 << kv.kv_shift, box = min(in_page, TILE_ROWS);
-            typename Ti::Ring r{bars, ring};
-            const auto put = [&](const CUtensorMap* map, int j) {
-                r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
-                    for (int a = 0; a < TILE_ROWS; a += box) {
-                        // rows behind the prefix and pages outside the cache: page -1, which the copy fills with zeros
-                        const int t = (j0 + j) * TILE_ROWS + a;
-                        int page = t < prefix ? pages[t >> kv.kv_shift] : -1;
-                        if ((unsigned)page >= (unsigned)kv.n_pages) page = -1;
-                        for (int c = 0; c < SC / CHUNK; ++c)
-                            tma_4d(dst + c * CHUNK_BYTES + a * 128, map, p * SC + c * CHUNK, kh, t & (in_page - 1), page, bar);
-                    }
-                });
-            };
-            put(&mk, 0);
-            for (int j = 0; j < n_all; ++j) {
-                if (j + 1 < n_all) put(&mk, j + 1);
-                put(&mv, j);
-            }
+        // A tile is 128 / box boxes, lane a issues box a (box: the rows of a page, at most 128). The pages of a tile are looked
+        // up two tiles ahead: one lane walking the list in line with its copies waited a memory latency per box (pages of 16
+        // rows: 6 us a tile). Rows behind the prefix and pages outside the cache: page -1, which the copy fills with zeros.
+        const int in_page = 1 << kv.kv_shift, box = min(in_page, TILE_ROWS), boxes = TILE_ROWS / box;
+        const auto page_of = [&](int j) {
+            const int t = (j0 + j) * TILE_ROWS + lane * box;
+            if (lane >= boxes || j >= n_all || t >= prefix) return -1;
+            const int p = pages[t >> kv.kv_shift];
+            return (unsigned)p < (unsigned)kv.n_pages ? p : -1;
+        };
+        typename Ti::Ring r{bars, ring};
+        const auto put = [&](const CUtensorMap* map, int j, int page) {
+            const int row = ((j0 + j) * TILE_ROWS + lane * box) & (in_page - 1);
+            r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
+                if (lane < boxes)
+                    for (int c = 0; c < SC / CHUNK; ++c)
+                        tma_4d(dst + c * CHUNK_BYTES + lane * box * 128, map, p * SC + c * CHUNK, kh, row, page, bar);
+            });
+        };
+        int p0 = page_of(0), p1 = page_of(1), p2 = page_of(2);
+        put(&mk, 0, p0);
+        for (int j = 0; j < n_all; ++j) {
+            const int p3 = page_of(j + 3);
+            if (j + 1 < n_all) put(&mk, j + 1, p1);
+            put(&mv, j, p0);
+            p0 = p1;
+            p1 = p2;
+            p2 = p3;
         }
     } else if (warp == NQ * 4) {
         Ti::few_registers();
@@ -89,29 +97,39 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
         const int i = warp >> 2, mine = r0 + warp * 32;     // this warp's 32 query rows
         // ---- queries to shared memory, a row of D values by the whole warp: K-major, 128-byte swizzle
         float c_row = 0.0f;
-#pragma unroll 4
-        for (int rr = 0; rr < 32; ++rr) {
-            const int r = mine + rr;
-            float v[N];
+        for (int r8 = 0; r8 < 32; r8 += 8) {      // eight rows in flight
+            float v[8][N], top[8];
 #pragma unroll
-            for (int e = 0; e < N; ++e) v[e] = 0.0f;
-            if (r < M) load_vals(q + ((long long)(r / G) * n_q + kh * G + r % G) * D + lane * N, v);
-            float top = 0.0f;
+            for (int t = 0; t < 8; ++t) {
+                const int r = mine + r8 + t;
 #pragma unroll
-            for (int e = 0; e < N; ++e) top = fmaxf(top, fabsf(v[e]));
+                for (int e = 0; e < N; ++e) v[t][e] = 0.0f;
+                if (r < M) load_vals(q + ((long long)(r / G) * n_q + kh * G + r % G) * D + lane * N, v[t]);
+            }
 #pragma unroll
-            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            const int x = q_exponent(top);
-            if (lane == rr) c_row = ldexpf(scale2, -x);
-            const int col = lane * N, in_tile = (warp & 3) * 32 + rr;
-            unsigned char* at = smem + i * Ti::QTILE * (SPLIT ? 2 : 1) + col / CHUNK * CHUNK_BYTES + in_tile * 128 +
-                                (((col % CHUNK / 8) ^ (in_tile & 7)) * 16) + col % 8 * 2;
+            for (int t = 0; t < 8; ++t) {
+                top[t] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < N; e += 2) {
-                uint32_t hi, lo;
-                split16(ldexpf(v[e], x), ldexpf(v[e + 1], x), &hi, &lo);
-                *reinterpret_cast<uint32_t*>(at + e * 2) = hi;
-                if constexpr (SPLIT) *reinterpret_cast<uint32_t*>(at + Ti::QTILE + e * 2) = lo;
+                for (int e = 0; e < N; ++e) top[t] = fmaxf(top[t], fabsf(v[t][e]));
+            }
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1)
+#pragma unroll
+                for (int t = 0; t < 8; ++t) top[t] = fmaxf(top[t], __shfl_xor_sync(0xffffffffu, top[t], off));
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                const int x = q_exponent(top[t]);
+                if (lane == r8 + t) c_row = ldexpf(scale2, -x);
+                const int col = lane * N, in_tile = (warp & 3) * 32 + r8 + t;
+                unsigned char* at = smem + i * Ti::QTILE * (SPLIT ? 2 : 1) + col / CHUNK * CHUNK_BYTES + in_tile * 128 +
+                                    (((col % CHUNK / 8) ^ (in_tile & 7)) * 16) + col % 8 * 2;
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    uint32_t hi, lo;
+                    split16(ldexpf(v[t][e], x), ldexpf(v[t][e + 1], x), &hi, &lo);
+                    *reinterpret_cast<uint32_t*>(at + e * 2) = hi;
+                    if constexpr (SPLIT) *reinterpret_cast<uint32_t*>(at + Ti::QTILE + e * 2) = lo;
+                }
             }
         }
         fence_async_smem();

@@ -65,24 +65,23 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     if (warp == NQ * 4 + 1) {
         Ti::few_registers();
         // ---- copies: Q, then K and V tiles in the order the tensor cores take them
+        const int kh = h / G, n_all = max(n[0], n[1]);
         if (lane == 0) {
-            const int kh = h / G, n_all = max(n[0], n[1]);
             mbar_expect(&bars.q_full, (n[1] ? 2 : 1) * Ti::QTILE);
             for (int i = 0; i < (n[1] ? 2 : 1); ++i)
                 for (int c = 0; c < D / CHUNK; ++c)
                     tma_3d(smem + i * Ti::QTILE + c * CHUNK_BYTES, &mq, c * CHUNK, h, q0 + i * TILE_ROWS, &bars.q_full);
-            typename Ti::Ring r{bars, ring};
-            const auto put = [&](const CUtensorMap* map, int j) {
-                r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
-                    for (int c = 0; c < SC / CHUNK; ++c)
-                        tma_3d(dst + c * CHUNK_BYTES, map, p * SC + c * CHUNK, kh, first + j * TILE_ROWS, bar);
-                });
-            };
-            put(&mk, 0);
-            for (int j = 0; j < n_all; ++j) {
-                if (j + 1 < n_all) put(&mk, j + 1);
-                put(&mv, j);
-            }
+        }
+        typename Ti::Ring r{bars, ring};
+        const auto put = [&](const CUtensorMap* map, int j) {
+            r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
+                if (lane < SC / CHUNK) tma_3d(dst + lane * CHUNK_BYTES, map, p * SC + lane * CHUNK, kh, first + j * TILE_ROWS, bar);
+            });
+        };
+        put(&mk, 0);
+        for (int j = 0; j < n_all; ++j) {
+            if (j + 1 < n_all) put(&mk, j + 1);
+            put(&mv, j);
         }
     } else if (warp == NQ * 4) {
         Ti::few_registers();

@@ -87,7 +87,8 @@ struct Tiles {
         if (threadIdx.x == 0 && bars.dead) atomicAdd(&attn_gave_up, 1);
     }
 
-    // The ring as the copying thread sees it: `load(smem, part, bar)` issues the copies of one stage
+    // The ring as the copying warp sees it: `load(smem, part, bar)` issues the copies of one stage, each lane its share of
+    // them. One lane waits, so that all of them go on or stop together.
     struct Ring {
         TileBars& bars;
         unsigned char* ring;
@@ -95,8 +96,12 @@ struct Tiles {
         template <typename F>
         __device__ __forceinline__ void put(F load) {
             for (int p = 0; p < PARTS; ++p) {
-                if (!wait_or_die(&bars.empty[st], ph ^ 1, &bars.dead)) return;
-                mbar_expect(&bars.full[st], STAGE);
+                int ok = 0;
+                if ((threadIdx.x & 31) == 0) {
+                    ok = wait_or_die(&bars.empty[st], ph ^ 1, &bars.dead);
+                    if (ok) mbar_expect(&bars.full[st], STAGE);
+                }
+                if (!__shfl_sync(0xffffffffu, ok, 0)) return;
                 load(ring + st * STAGE, p, &bars.full[st]);
                 if (++st == ST) { st = 0; ph ^= 1; }
             }
