@@ -230,10 +230,9 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                 if (k >= k1 || r >= own) return -1;
                 if constexpr (!BOX) return kv.row(b, start + r);
                 const int* list = kv.pages + (long long)b * kv.max_pages + ((start + r) >> kv.kv_shift);
-                const unsigned p0 = list[0], n = kv.n_pages;
-                unsigned p1 = n;
-                if (kv.kv_shift == 3 && r + 8 < own) p1 = list[1];
-                return ((long long)(p1 < n ? p1 : -1) << 32) | (unsigned)(p0 < n ? p0 : -1);
+                const auto valid = [&](int p) { return (unsigned)p < (unsigned)kv.n_pages ? p : -1; };
+                const int p0 = valid(list[0]), p1 = kv.kv_shift == 3 && r + 8 < own ? valid(list[1]) : -1;
+                return ((long long)p1 << 32) | (unsigned)p0;
             };
             unsigned seen[ST];       // which rows of a stage hold a row of the sequence (indexed by unrolled stages only)
             const auto fetch = [&](int s, int k, long long at) -> unsigned {
@@ -293,7 +292,7 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                         unsigned char* Kt = ring + s * Sh::STAGE;
                         unsigned char* Vt = Kt + 16 * D * 2;
                         if constexpr (BOX) {
-                            if (alive) alive = mbar_wait(&full[warp][s], phases >> s & 1);
+                            if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&full[warp][s], phases >> s & 1));
                             phases ^= 1u << s;
                             if (seen[s] != 0xffffu) {   // a weight of 0 needs a finite v: what lies behind the sequence is blanked
                                 for (int e = lane; e < 16 * UNITS; e += 32)

@@ -34,12 +34,12 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
     __shared__ TileBars bars;
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     unsigned char* ring = smem + Ti::Q_BYTES;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = n_q / n_kv;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31, G = n_q / n_kv;
     if (warp == NQ * 4 + 1 && lane == 0) {
         tma_prefetch(&mk);
         tma_prefetch(&mv);
     }
-    Ti::setup(bars, NQ * 4);
+    Ti::setup(bars, 4);
     // No wait for the kernel before this one (k_attn_own) here: it began after its own predecessors were done, it writes
     // nothing that is read here, and this kernel starts only once all of its CTAs have begun. The wait at the end makes
     // this kernel's completion stand for both.
@@ -91,7 +91,8 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
         }
     } else if (warp == NQ * 4) {
         Ti::few_registers();
-        if (lane == 0) Ti::products(bars, smem, ring, n);
+        TileFlow f;
+        Ti::products(bars, smem, ring, n[0], n[1], f);
     } else if (warp < NQ * 4) {
         Ti::many_registers();
         const int i = warp >> 2, mine = r0 + warp * 32;     // this warp's 32 query rows
@@ -134,7 +135,7 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.q_full);
+        if (lane == 0) mbar_arrive(&bars.q_full[i]);
 
         float m = -INFINITY, l = 0.0f;
         const int tiles_i = i ? n[1] : n[0];
@@ -144,18 +145,19 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             return j < tiles_i && t < prefix && (unsigned)pages[t >> kv.kv_shift] < (unsigned)kv.n_pages;
         };
         bool next = look(0);
+        TileFlow f;
         for (int j = 0; j < tiles_i; ++j) {
             const unsigned seen = __ballot_sync(0xffffffffu, next);
             next = look(j + 1);
             uint32_t x[128];
-            if (!Ti::scores(bars, i, j, x)) break;
+            if (!Ti::scores(bars, i, f, x)) break;
             if (seen != 0xffffffffu)
 #pragma unroll
                 for (int e = 0; e < 128; ++e)
                     if (!(seen >> (e / 4) & 1)) x[e] = 0xff800000u;
-            if (!Ti::weights(bars, i, j, x, c_row, m, l)) break;
+            if (!Ti::weights(bars, i, j == 0, j + 1 == tiles_i, f, x, c_row, m, l)) break;
         }
-        if (tiles_i > 0 && wait_or_die(&bars.o_full[i], 0, &bars.dead)) {
+        if (tiles_i > 0 && warp_wait(&bars.o_full[i], 0, &bars.dead)) {
             tc_fence_after();
             const uint32_t o_addr = bars.tmem + 256 + i * D + ((uint32_t)(threadIdx.x & 96) << 16);
             const long long at = ((long long)split * n_kv + kh) * px.rows + mine;

@@ -16,6 +16,41 @@ template <int D, typename T>
 using PromptTiles = Tiles<D, D == 256 ? 1 : 2, D < 128 ? D : 128, D == 64 ? 8 : 5, false, T>;
 __host__ __device__ constexpr int prompt_rows(int D) { return D == 256 ? TILE_ROWS : 2 * TILE_ROWS; }   // query rows of a CTA
 
+// What a CTA works on next: up to ROWS query rows of one head of one sequence
+struct PromptItem {
+    int h, first, q0, end;      // head; the sequence's first row; the first query row; the sequence's end
+    int n[2];                   // key tiles per query tile; n[0] == 0: there is nothing more
+};
+struct PromptBars {
+    unsigned long long item_full[2], item_empty[2], q_empty[2], asked;
+    uint4 answer;               // of the work distributor, 16 bytes
+    PromptItem item[2];
+};
+
+// The next block of the grid that has not begun, taken over by this CTA (the hardware's work distributor hands blocks to CTAs
+// that ask as it hands them to SMs that are free): asks, and later reads the answer. One thread.
+__device__ __forceinline__ void ask_for_block(PromptBars& pb) {
+    mbar_expect(&pb.asked, 16);
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+                 ::"r"(smem_u32(&pb.answer)), "r"(smem_u32(&pb.asked))
+                 : "memory");
+}
+__device__ __forceinline__ int block_answer(PromptBars& pb) {   // the block's index, -1: there is none
+    int got, x;
+    asm volatile("{\n\t.reg .b128 r;\n\t.reg .pred p;\n\tld.shared.b128 r, [%2];\n\t"
+                 "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\tselp.s32 %0, 1, 0, p;\n\tmov.s32 %1, 0;\n\t"
+                 "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+                 : "=r"(got), "=r"(x)
+                 : "r"(smem_u32(&pb.answer))
+                 : "memory");
+    return got ? x : -1;
+}
+
+// The grid is all blocks of work, heaviest first as far as one pass over the batch knows; a CTA that has finished one takes
+// the next that nobody has begun. Its roles run ahead of one another: while the softmax warps still write one block's rows,
+// the schedule warp has looked up the next block, its first K and V tiles are on their way, and the tensor cores begin as
+// soon as the query tile's memory is free. (One CTA per block: 61 sequences of 200 rows, 16 heads of 64, took 98 us, most of
+// it the way from a CTA's start to its first product and from its last to its end.)
 template <int D, typename T>
 __global__ void __launch_bounds__(PromptTiles<D, T>::WARPS * 32, 1)
 k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -25,83 +60,156 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     constexpr int NQ = D == 256 ? 1 : 2, SC = D < 128 ? D : 128, ROWS = prompt_rows(D);
     extern __shared__ unsigned char smem_raw[];
     __shared__ TileBars bars;
+    __shared__ PromptBars pb;
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     unsigned char* ring = smem + Ti::Q_BYTES;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (warp == NQ * 4 + 1 && lane == 0) {
         tma_prefetch(&mq);
         tma_prefetch(&mk);
         tma_prefetch(&mv);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&pb.item_full[i], 1);
+            mbar_init(&pb.item_empty[i], NQ * 4 + 2);
+            mbar_init(&pb.q_empty[i], 4);
+        }
+        mbar_init(&pb.asked, 1);
+        mbar_fence_init();
     }
     Ti::setup(bars, 1);
     pdl_entry();
 
-    // which rows: slot s of the packed batch is tile s - f(b) of sequence b, f(b) = floor(start(b) / ROWS) + b, the last b with
-    // f(b) <= s; f(b + 1) - f(b) is at least the number of tiles b has. Slots are taken from the last one down, so that in a
-    // long sequence the tiles with the most keys start first.
-    const int h = blockIdx.x % n_q, slot = n_slots - 1 - blockIdx.x / n_q;
-    int first = 0, end = rows, tile = slot;
-    if (seq_start) {
-        int lo = 0, hi = n_seqs;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
-            if (min(max(seq_start[mid], 0), rows) / ROWS + mid <= slot) lo = mid + 1; else hi = mid;
-        }
-        const int b = max(lo - 1, 0);
-        first = min(max(seq_start[b], 0), rows);
-        end = min(seq_start[b + 1], rows);
-        tile = slot - (first / ROWS + b);
-    }
-    const int q0 = tile < 0 || tile > (end - first) / ROWS ? end : first + tile * ROWS;   // (no overflow on bad borders)
-    if (q0 < end) {
-    // key tiles per query tile: those up to its last row's own place
-    int n[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int a = q0 + i * TILE_ROWS;
-        n[i] = i < NQ && a < end ? (min(a + TILE_ROWS, end) - 1 - first) / TILE_ROWS + 1 : 0;
-    }
+    // the consumers' side of the items: what to do next, until n[0] is 0
+    unsigned taken = 0;
+    const auto next_item = [&](PromptItem* it) {
+        const int slot = taken & 1;
+        if (!warp_wait(&pb.item_full[slot], taken >> 1 & 1, &bars.dead)) return false;
+        *it = pb.item[slot];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&pb.item_empty[slot]);
+        ++taken;
+        return it->n[0] > 0;
+    };
 
-    if (warp == NQ * 4 + 1) {
+    if (warp == NQ * 4 + 2) {
         Ti::few_registers();
-        // ---- copies: Q, then K and V tiles in the order the tensor cores take them
-        const int kh = h / G, n_all = max(n[0], n[1]);
-        if (lane == 0) {
-            mbar_expect(&bars.q_full, (n[1] ? 2 : 1) * Ti::QTILE);
-            for (int i = 0; i < (n[1] ? 2 : 1); ++i)
-                for (int c = 0; c < D / CHUNK; ++c)
-                    tma_3d(smem + i * Ti::QTILE + c * CHUNK_BYTES, &mq, c * CHUNK, h, q0 + i * TILE_ROWS, &bars.q_full);
+        // ---- schedule: blocks of work, two ahead of the CTA's slowest role
+        int block = blockIdx.x;
+        unsigned made = 0, asked = 0;
+        while (true) {
+            // (the next answer is under way while this block is looked up)
+            if (block >= 0 && lane == 0) ask_for_block(pb);
+            PromptItem it = {0, 0, 0, 0, {0, 0}};
+            if (block >= 0) {
+                // slot s of the packed batch is tile s - f(b) of sequence b, f(b) = floor(start(b) / ROWS) + b, the last b with
+                // f(b) <= s; f(b + 1) - f(b) is at least the number of tiles b has. Slots are taken from the last one down, so
+                // that in a sequence the tiles with the most keys come first.
+                const int slot = n_slots - 1 - block / n_q;
+                int first = 0, end = rows, tile = slot;
+                if (seq_start) {
+                    int lo = 0, hi = n_seqs;            // the last b with f(b) <= slot is in [lo - 1, hi): 32 probes a step
+                    while (lo < hi) {
+                        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+                        const bool yes = at < hi && min(max(seq_start[at], 0), rows) / ROWS + at <= slot;
+                        const unsigned votes = __ballot_sync(0xffffffffu, yes);
+                        const int k = votes ? 32 - __clz(votes) : 0;      // probes up to k - 1 hold
+                        if (k == 0) { hi = lo; break; }
+                        const int base = lo + (k - 1) * step;             // holds; the answer is in [base, base + step)
+                        lo = base + 1;
+                        hi = min(base + step, hi);
+                    }
+                    const int b = max(lo - 1, 0);
+                    first = min(max(seq_start[b], 0), rows);
+                    end = min(seq_start[b + 1], rows);
+                    tile = slot - (first / ROWS + b);
+                }
+                if (tile >= 0 && tile <= (end - first) / ROWS && first + tile * ROWS < end) {   // (no overflow on bad borders)
+                    it.h = block % n_q;
+                    it.first = first;
+                    it.q0 = first + tile * ROWS;
+                    it.end = end;
+#pragma unroll
+                    for (int i = 0; i < NQ; ++i) {      // those up to the last row's own place
+                        const int a = it.q0 + i * TILE_ROWS;
+                        it.n[i] = a < end ? (min(a + TILE_ROWS, end) - 1 - first) / TILE_ROWS + 1 : 0;
+                    }
+                }
+            }
+            if (it.n[0] > 0 || block < 0) {
+                const int s = made & 1;
+                if (!warp_wait(&pb.item_empty[s], made >> 1 & 1 ^ 1, &bars.dead)) break;
+                if (lane == 0) {
+                    pb.item[s] = it;
+                    mbar_arrive(&pb.item_full[s]);
+                }
+                ++made;
+            }
+            if (block < 0) break;
+            if (!warp_wait(&pb.asked, asked & 1, &bars.dead)) break;
+            ++asked;
+            block = block_answer(pb);
+            fence_async_smem();          // the answer has been read before the next one may arrive
+            __syncwarp();
         }
+    } else if (warp == NQ * 4 + 1) {
+        Ti::few_registers();
+        // ---- copies: K and V tiles in the order the tensor cores take them, and Q as soon as its place is free
         typename Ti::Ring r{bars, ring};
-        const auto put = [&](const CUtensorMap* map, int j) {
-            r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
-                if (lane < SC / CHUNK) tma_3d(dst + lane * CHUNK_BYTES, map, p * SC + lane * CHUNK, kh, first + j * TILE_ROWS, bar);
-            });
-        };
-        put(&mk, 0);
-        for (int j = 0; j < n_all; ++j) {
-            if (j + 1 < n_all) put(&mk, j + 1);
-            put(&mv, j);
+        PromptItem it;
+        unsigned items[2] = {0, 0};
+        while (next_item(&it)) {
+            const int kh = it.h / G, n_all = max(it.n[0], it.n[1]);
+            const auto put = [&](const CUtensorMap* map, int j) {
+                r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
+                    if (lane < SC / CHUNK) tma_3d(dst + lane * CHUNK_BYTES, map, p * SC + lane * CHUNK, kh, it.first + j * TILE_ROWS, bar);
+                });
+            };
+            put(&mk, 0);
+#pragma unroll
+            for (int i = 0; i < NQ; ++i) {
+                if (it.n[i] == 0) continue;
+                if (!warp_wait(&pb.q_empty[i], items[i] & 1 ^ 1, &bars.dead)) break;
+                ++items[i];
+                if (lane == 0) mbar_expect(&bars.q_full[i], Ti::QTILE);
+                __syncwarp();
+                if (lane < D / CHUNK)
+                    tma_3d(smem + i * Ti::QTILE + lane * CHUNK_BYTES, &mq, lane * CHUNK, it.h, it.q0 + i * TILE_ROWS, &bars.q_full[i]);
+            }
+            for (int j = 0; j < n_all; ++j) {
+                if (j + 1 < n_all) put(&mk, j + 1);
+                put(&mv, j);
+            }
         }
     } else if (warp == NQ * 4) {
         Ti::few_registers();
-        if (lane == 0) Ti::products(bars, smem, ring, n);
+        TileFlow f;
+        PromptItem it;
+        while (next_item(&it))
+            if (!Ti::products(bars, smem, ring, it.n[0], it.n[1], f)) break;
     } else if (warp < NQ * 4) {
         Ti::many_registers();
         // ---- softmax: thread = row
-        const int i = warp >> 2, r = threadIdx.x & 127, row = q0 + i * TILE_ROWS + r, tiles = i ? n[1] : n[0];
-        float m = -INFINITY, l = 0.0f;
-        for (int j = 0; j < tiles; ++j) {
-            uint32_t x[128];
-            if (!Ti::scores(bars, i, j, x)) break;
-            const int last = row - first - j * TILE_ROWS;   // the last key of this tile that the row sees
-            if (j + 1 == tiles)   // (uniform) only a query tile's last key tile reaches past any of its rows
+        const int i = warp >> 2, r = threadIdx.x & 127;
+        TileFlow f;
+        PromptItem it;
+        while (next_item(&it)) {
+            const int tiles = i ? it.n[1] : it.n[0], h = it.h, first = it.first, end = it.end, t0 = it.q0 + i * TILE_ROWS, row = t0 + r;
+            if (tiles == 0) continue;
+            float m = -INFINITY, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < tiles && ok; ++j) {
+                uint32_t x[128];
+                ok = Ti::scores(bars, i, f, x);
+                if (!ok) break;
+                const int last = row - first - j * TILE_ROWS;   // the last key of this tile that the row sees
+                if (j + 1 == tiles)   // (uniform) only a query tile's last key tile reaches past any of its rows
 #pragma unroll
-                for (int c = 0; c < 128; ++c)
-                    if (c > last) x[c] = 0xff800000u;
-            if (!Ti::weights(bars, i, j, x, scale2, m, l)) break;
-        }
-        if (tiles > 0 && wait_or_die(&bars.o_full[i], 0, &bars.dead)) {
+                    for (int c = 0; c < 128; ++c)
+                        if (c > last) x[c] = 0xff800000u;
+                ok = Ti::weights(bars, i, j == 0, j + 1 == tiles, f, x, scale2, m, l);
+            }
+            if (!ok || !warp_wait(&bars.o_full[i], f.items[0] & 1, &bars.dead)) break;
+            ++f.items[0];
             tc_fence_after();
             // O / l through the Q tile's shared memory (its last S is done), so that whole rows leave the warp together
             const uint32_t o_addr = bars.tmem + 256 + i * D + ((uint32_t)(threadIdx.x & 96) << 16);
@@ -115,30 +223,33 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 tmem_pin(o);
 #pragma unroll
                 for (int e = 0; e < 32; e += 8) {
-                    float f[8];
+                    float y[8];
 #pragma unroll
                     for (int t = 0; t < 8; ++t) {
-                        f[t] = __uint_as_float(o[e + t]) * inv;
-                        bad |= !(fabsf(f[t]) < INFINITY);
+                        y[t] = __uint_as_float(o[e + t]) * inv;
+                        bad |= !(fabsf(y[t]) < INFINITY);
                     }
                     const int u = (c + e) / 8;
-                    *reinterpret_cast<uint4*>(mine + lane * (D * 2) + ((u ^ (lane & 7)) * 16)) = Io<T>::pack(f);
+                    *reinterpret_cast<uint4*>(mine + lane * (D * 2) + ((u ^ (lane & 7)) * 16)) = Io<T>::pack(y);
                 }
             }
             __syncwarp();
             constexpr int UNITS = D / 8;
+#pragma unroll 4
             for (int e = lane; e < 32 * UNITS; e += 32) {
-                const int rr = e / UNITS, u = e % UNITS, t = q0 + i * TILE_ROWS + (warp & 3) * 32 + rr;
-                if (t < end)
-                    st_stream(reinterpret_cast<unsigned char*>(out + ((long long)t * n_q + h) * D) + u * 16,
-                              *reinterpret_cast<const uint4*>(mine + rr * (D * 2) + ((u ^ (rr & 7)) * 16)));
+                const int rr = e / UNITS, u = e % UNITS, t = t0 + (warp & 3) * 32 + rr;
+                const uint4 y = *reinterpret_cast<const uint4*>(mine + rr * (D * 2) + ((u ^ (rr & 7)) * 16));
+                if (t < end) st_stream(reinterpret_cast<unsigned char*>(out + ((long long)t * n_q + h) * D) + u * 16, y);
             }
+            // the query tile's memory may take the next one
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pb.q_empty[i]);
             // A weight of 0 times a non-finite v is not 0 on the tensor cores: rows that came out non-finite are computed again
             // from the keys they may see alone
             unsigned again = __ballot_sync(0xffffffffu, bad && row < end);
-            __syncwarp();
             while (again) {
-                const int rr = __ffs(again) - 1, t = q0 + i * TILE_ROWS + (warp & 3) * 32 + rr;
+                const int t = t0 + (warp & 3) * 32 + __ffs(again) - 1;
                 again &= again - 1;
                 attn_row_prompt<D, T>(q + t * q_stride + h * D, k + first * k_stride + h / G * D, v + first * v_stride + h / G * D,
                                       k_stride, v_stride, t - first + 1, scale2, out + ((long long)t * n_q + h) * D);
@@ -146,7 +257,6 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         }
     } else {
         Ti::few_registers();
-    }
     }
     Ti::teardown(bars);
 }

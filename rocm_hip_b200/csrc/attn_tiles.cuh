@@ -21,17 +21,38 @@ namespace b200 {
 __device__ int attn_gave_up;
 
 struct TileBars {
-    unsigned long long q_full, s_full[2], p_full[2], o_full[2], o_part, full[8], empty[8];
+    unsigned long long q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_part, full[8], empty[8];
     uint32_t tmem;
     int dead;
 };
 
-// A wait that gives up for the whole CTA: once one role is dead nobody waits or issues any more
+// Where a role stands: barriers count on over all the query tiles a CTA works through. steps: key tiles per query tile (NQ = 1:
+// of the CTA, whose two S buffers take turns); items: query tiles; parts: products that were not a query tile's last.
+struct TileFlow {
+    int stage = 0, phase = 0;
+    unsigned steps[2] = {0, 0}, items[2] = {0, 0}, parts = 0;
+};
+
+// A wait that gives up for the whole CTA: once one role is dead nobody waits or issues any more. `dead` is looked at only
+// while the barrier is not there yet.
 __device__ __forceinline__ bool wait_or_die(unsigned long long* bar, unsigned parity, volatile int* dead) {
-    if (*dead) return false;
-    if (mbar_wait(bar, parity)) return true;
+    const unsigned b = smem_u32(bar);
+    for (int i = 0; i < MBAR_POLLS; ++i) {
+        unsigned ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(b), "r"(parity)
+                     : "memory");
+        if (ok) return true;
+        if (*dead) return false;
+    }
     *dead = 1;
     return false;
+}
+
+// the same for a whole warp: all lanes go on, or none
+__device__ __forceinline__ bool warp_wait(unsigned long long* bar, unsigned parity, volatile int* dead) {
+    return __all_sync(0xffffffffu, wait_or_die(bar, parity, dead));
 }
 
 // SC: columns of a ring stage (a K or V tile is D / SC stages of 128 rows), ST: stages
@@ -42,7 +63,11 @@ struct Tiles {
     static constexpr int QTILE = TILE_ROWS * D * 2;                        // one query tile, one half of a split one
     static constexpr int Q_BYTES = NQ * QTILE * (SPLIT ? 2 : 1);           // [NQ][hi, lo][D / 64][128 rows][64 values]
     static constexpr int SMEM = 1024 + Q_BYTES + ST * STAGE;
-    static constexpr int WARPS = NQ == 2 ? 12 : 6;                         // softmax, tensor cores, copies (and two idle warps)
+    static constexpr int WARPS = NQ == 2 ? 12 : 7;                         // softmax, tensor cores, copies, schedule (and an idle one)
+    // NQ = 2: the products of a tile's first half of the keys begin while the second half is still in the softmax (8,192 rows,
+    // 32 heads of 128: 1,246 -> 1,295 TFLOP/s). With one query tile the next S fills that time (heads of 256: 1,286 without,
+    // 1,261 with).
+    static constexpr bool HALVES = NQ == 2;
     static constexpr int P_SHIFT_T = std::is_same<T, __half>::value ? 7 : 0;   // fp16 weights are held times 2^7 (at most 2^15)
 
     // A softmax thread holds its row's 128 scores: 208 registers. Twelve warps start with 168 each (64,512 in all); the four
@@ -55,16 +80,17 @@ struct Tiles {
         if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     }
 
-    // Barriers and tensor memory; all threads. q_arrivals: who fills the query tiles.
+    // Barriers and tensor memory; all threads. q_arrivals: how many fill a query tile.
     static __device__ __forceinline__ void setup(TileBars& bars, int q_arrivals) {
         const int warp = threadIdx.x >> 5;
         if (warp == NQ * 4) {
             tmem_alloc(&bars.tmem, 512);
             if ((threadIdx.x & 31) == 0) {
-                mbar_init(&bars.q_full, q_arrivals);
                 mbar_init(&bars.o_part, 1);
                 for (int i = 0; i < 2; ++i) {
+                    mbar_init(&bars.q_full[i], q_arrivals);
                     mbar_init(&bars.s_full[i], 1);
+                    mbar_init(&bars.p_half[i], 4);
                     mbar_init(&bars.p_full[i], 4);
                     mbar_init(&bars.o_full[i], 1);
                 }
@@ -108,77 +134,116 @@ struct Tiles {
         }
     };
 
-    // One thread: everything the tensor cores do for n[0] / n[1] key tiles of the query tiles. The ring brings
-    // K 0, K 1, V 0, K 2, V 1, ...
-    static __device__ __forceinline__ void products(TileBars& bars, const unsigned char* qs, const unsigned char* ring, const int (&n)[2]) {
-        const uint32_t tmem = bars.tmem, id_s = idesc_f16<T>(TILE_ROWS, false), id_o = idesc_f16<T>(SC, true);
-        const int n_all = max(n[0], n[1]);
-        int st = 0, ph = 0;                   // the next stage to be taken from the ring
-        const auto take = [&](int* stage) {   // the stages of a tile
+    static __device__ __forceinline__ int buffer(unsigned steps, int i) { return NQ == 1 ? steps & 1 : i; }
+    static __device__ __forceinline__ unsigned parity(unsigned steps) { return NQ == 1 ? steps >> 1 & 1 : steps & 1; }
+
+    // One warp: everything the tensor cores do for n0 / n1 key tiles of the query tiles. The ring brings
+    // K 0, K 1, V 0, K 2, V 1, ...  False: given up.
+    static __device__ __forceinline__ bool products(TileBars& bars, const unsigned char* qs, const unsigned char* ring, int n0, int n1,
+                                                    TileFlow& f) {
+        constexpr uint32_t id_s = idesc_f16<T>(TILE_ROWS, false), id_o = idesc_f16<T>(SC, true);
+        constexpr int Z = SPLIT ? 2 : 1;
+        const uint32_t tmem = bars.tmem, q_desc = desc_k_major(smem_u32(qs)), k_desc = desc_k_major(smem_u32(ring)),
+                       v_desc = desc_mn_major(smem_u32(ring));
+        const int n_all = max(n0, n1);
+        bool dead = false;
+        const auto after = [](int stage, int p) { return stage + p < ST ? stage + p : stage + p - ST; };
+        const auto take = [&]() {             // the stages of a tile: the first one
+            const int first = f.stage;
+#pragma unroll
             for (int p = 0; p < PARTS; ++p) {
-                stage[p] = st;
-                wait_or_die(&bars.full[st], ph, &bars.dead);
-                if (++st == ST) { st = 0; ph ^= 1; }
+                dead = dead || !warp_wait(&bars.full[f.stage], f.phase, &bars.dead);
+                if (++f.stage == ST) { f.stage = 0; f.phase ^= 1; }
             }
             tc_fence_after();
+            return first;
         };
-        const auto give = [&](const int* stage) {
-            for (int p = 0; p < PARTS; ++p) mma_commit(&bars.empty[stage[p]]);
+        const auto give = [&](int stage) {
+            if (elect_one())
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) mma_commit(&bars.empty[after(stage, p)]);
         };
-        const auto score = [&](int i, int buf, const int* stage) {   // S[buf] = Q_i K^T
-            if (bars.dead) return;
-            for (int c = 0; c < D / CHUNK; ++c) {
-                const uint64_t b = desc_k_major(smem_u32(ring) + stage[c / (SC / CHUNK)] * STAGE + c % (SC / CHUNK) * CHUNK_BYTES);
-                for (int z = 0; z < (SPLIT ? 2 : 1); ++z) {
-                    const uint64_t a = desc_k_major(smem_u32(qs) + (i * (SPLIT ? 2 : 1) + z) * QTILE + c * CHUNK_BYTES);
-                    for (int e = 0; e < CHUNK / 16; ++e) mma_ss(tmem + buf * 128, a + e * 2, b + e * 2, id_s, c + e + z > 0);
+        const auto score = [&](int i, int buf, int stage) {   // S[buf] = Q_i K^T
+            const uint32_t d = tmem + buf * 128;
+            if (elect_one()) {
+#pragma unroll
+                for (int c = 0; c < D / CHUNK; ++c) {
+                    const uint32_t b = k_desc + after(stage, c / (SC / CHUNK)) * (STAGE >> 4) + c % (SC / CHUNK) * (CHUNK_BYTES >> 4);
+#pragma unroll
+                    for (int z = 0; z < Z; ++z) {
+                        const uint32_t a = q_desc + (i * Z + z) * (QTILE >> 4) + c * (CHUNK_BYTES >> 4);
+#pragma unroll
+                        for (int e = 0; e < CHUNK / 16; ++e) mma_ss(d, a + e * 2, b + e * 2, id_s, c + e + z > 0);
+                    }
+                }
+                mma_commit(&bars.s_full[buf]);
+            }
+        };
+        // O_i += P[buf] V for the 16-key steps [e0, e1)
+        const auto join = [&](int i, int buf, int stage, bool add, int e0, int e1) {
+            if (elect_one()) {
+#pragma unroll
+                for (int p = 0; p < PARTS; ++p) {
+                    const uint32_t b = v_desc + after(stage, p) * (STAGE >> 4), d = tmem + 256 + i * D + p * SC;
+#pragma unroll
+                    for (int z = 0; z < Z; ++z)
+#pragma unroll
+                        for (int e = e0; e < e1; ++e)
+                            mma_ts(d, tmem + buf * 128 + z * 64 + e * 8, b + e * (16 * 128 >> 4), id_o, add || e + z > e0);
                 }
             }
-            mma_commit(&bars.s_full[buf]);
         };
-        const auto join = [&](int i, int buf, const int* stage, bool add) {   // O_i += P[buf] V
-            if (bars.dead) return;
-            for (int p = 0; p < PARTS; ++p) {
-                const uint64_t b = desc_mn_major(smem_u32(ring) + stage[p] * STAGE);
-                for (int z = 0; z < (SPLIT ? 2 : 1); ++z)
-                    for (int e = 0; e < TILE_ROWS / 16; ++e)
-                        mma_ts(tmem + 256 + i * D + p * SC, tmem + buf * 128 + z * 64 + e * 8, b + e * (16 * 128 >> 4), id_o, add || e + z > 0);
-            }
-        };
-        wait_or_die(&bars.q_full, 0, &bars.dead);
-        tc_fence_after();
-        int ks[PARTS], vs[PARTS];
-        take(ks);
-        for (int i = 0; i < NQ; ++i)
-            if (n[i] > 0) score(i, NQ == 1 ? 0 : i, ks);
+        int ks = take(), vs;
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            if ((i ? n1 : n0) == 0) continue;
+            dead = dead || !warp_wait(&bars.q_full[i], f.items[i] & 1, &bars.dead);
+            if (dead) return false;
+            tc_fence_after();
+            score(i, buffer(f.steps[i], i), ks);
+        }
         give(ks);
         for (int j = 0; j < n_all; ++j) {
             const bool more = j + 1 < n_all;
-            if (more) take(ks);
+            if (more) ks = take();
+            if (dead) return false;
             if (NQ == 1 && more) {
-                score(0, (j + 1) & 1, ks);
+                score(0, buffer(f.steps[0] + 1, 0), ks);
                 give(ks);
             }
-            take(vs);
+            vs = take();
+#pragma unroll
             for (int i = 0; i < NQ; ++i) {
-                if (j >= n[i]) continue;
-                const int buf = NQ == 1 ? j & 1 : i;
-                wait_or_die(&bars.p_full[buf], NQ == 1 ? (j >> 1) & 1 : j & 1, &bars.dead);
+                const int ni = i ? n1 : n0, buf = buffer(f.steps[i], i);
+                if (j >= ni) continue;
+                if (HALVES) {
+                    dead = dead || !warp_wait(&bars.p_half[buf], parity(f.steps[i]), &bars.dead);
+                    if (dead) return false;
+                    tc_fence_after();
+                    join(i, buf, vs, j > 0, 0, 4);
+                }
+                dead = dead || !warp_wait(&bars.p_full[buf], parity(f.steps[i]), &bars.dead);
+                if (dead) return false;
                 tc_fence_after();
-                join(i, buf, vs, j > 0);
-                if (j + 1 == n[i]) mma_commit(&bars.o_full[i]);
-                else if (NQ == 1) mma_commit(&bars.o_part);
-                if (NQ == 2 && j + 1 < n[i]) score(i, i, ks);
+                join(i, buf, vs, HALVES || j > 0, HALVES ? 4 : 0, 8);
+                ++f.steps[i];
+                if (NQ == 1 || j + 1 == ni) {
+                    if (elect_one()) mma_commit(j + 1 == ni ? &bars.o_full[i] : &bars.o_part);
+                }
+                if (NQ == 2 && j + 1 < ni) score(i, i, ks);
             }
             if (NQ == 2 && more) give(ks);
             give(vs);
         }
+        if (n0 > 0) ++f.items[0];
+        if (n1 > 0) ++f.items[1];
+        return true;
     }
 
-    // A softmax thread: its row's scores against key tile j into x, once they are there
-    static __device__ __forceinline__ bool scores(TileBars& bars, int i, int j, uint32_t (&x)[128]) {
-        const int buf = NQ == 1 ? j & 1 : i;
-        if (!wait_or_die(&bars.s_full[buf], NQ == 1 ? (j >> 1) & 1 : j & 1, &bars.dead)) return false;
+    // A softmax thread: its row's scores against the next key tile into x, once they are there
+    static __device__ __forceinline__ bool scores(TileBars& bars, int i, const TileFlow& f, uint32_t (&x)[128]) {
+        const int buf = buffer(f.steps[0], i);
+        if (!warp_wait(&bars.s_full[buf], parity(f.steps[0]), &bars.dead)) return false;
         tc_fence_after();
         const uint32_t s_addr = bars.tmem + buf * 128 + ((uint32_t)(threadIdx.x & 96) << 16);
 #pragma unroll
@@ -189,19 +254,24 @@ struct Tiles {
         return true;
     }
 
-    // ... and, masked scores (-inf) in x, from there to P in tensor memory; c > 0 turns scores into powers of two
-    static __device__ __forceinline__ bool weights(TileBars& bars, int i, int j, uint32_t (&x)[128], float c, float& m, float& l) {
-        const int buf = NQ == 1 ? j & 1 : i;
+    // ... and, masked scores (-inf) in x, from there to P in tensor memory; c > 0 turns scores into powers of two. first / last: of
+    // the query tile's key tiles. (f.steps[0] counts this role's steps whichever query tile it has.)
+    static __device__ __forceinline__ bool weights(TileBars& bars, int i, bool first, bool last, TileFlow& f, uint32_t (&x)[128], float c,
+                                                   float& m, float& l) {
+        const int buf = buffer(f.steps[0], i);
         const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
         const uint32_t s_addr = bars.tmem + buf * 128 + lanes, o_addr = bars.tmem + 256 + i * D + lanes;
-        float mx = -INFINITY;
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains of three-way maxima
 #pragma unroll
-        for (int e = 0; e < 128; ++e) mx = fmaxf(mx, __uint_as_float(x[e]));
-        if (j == 0) m = mx;
+        for (int e = 0; e < 128; e += 8)
+#pragma unroll
+            for (int t = 0; t < 4; ++t) top[t] = max3(top[t], __uint_as_float(x[e + 2 * t]), __uint_as_float(x[e + 2 * t + 1]));
+        const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+        if (first) m = mx;
         else if (__any_sync(0xffffffffu, (mx - m) * c > 8.0f)) {
             // O holds the tiles before this one. NQ = 2: their products were issued before this S, so they are done. NQ = 1:
             // the last of them comes behind this S.
-            if (NQ == 1 && !wait_or_die(&bars.o_part, (j - 1) & 1, &bars.dead)) return false;
+            if (NQ == 1 && !warp_wait(&bars.o_part, (f.parts - 1) & 1, &bars.dead)) return false;
             tc_fence_after();
             const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : ex2((m - mn) * c);
             m = mn;
@@ -218,29 +288,46 @@ struct Tiles {
         }
         const float neg = m == -INFINITY ? 0.0f : P_SHIFT_T - m * c;
         const f2 neg2 = pk2(neg, neg), c2 = pk2(c, c);
-        f2 sum = pk2(0.0f, 0.0f);
+        // Of every EMU pairs one takes the polynomial: the special-function unit gives 16 values a clock and SM, two query tiles
+        // of 128-wide heads want 128 x 128 of them every 1,024 clocks, which is all of them (0, 3, 4, 6: 1,242, 1,272, 1,295 and
+        // 1,290 TFLOP/s), narrower heads more (64: 660, 731, 719 with 0, 3, 4); 256-wide heads half of them, and the
+        // polynomial's instructions only cost (1,325, 1,249, 1,286 with 0, 3, 4).
+        constexpr int EMU = SPLIT || NQ == 1 ? 0 : D == 64 ? 3 : 4;
+        f2 sum[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
 #pragma unroll
-        for (int e0 = 0; e0 < 128; e0 += 64) {
+        for (int half = 0; half < 2; ++half) {
             uint32_t p[32], lo[SPLIT ? 32 : 1];
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
+                const int at = half * 64 + 2 * e;
+                f2 w = fma2(pk2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), c2, neg2);
                 float a, b;
-                upk2(fma2(pk2(__uint_as_float(x[e0 + 2 * e]), __uint_as_float(x[e0 + 2 * e + 1])), c2, neg2), a, b);
-                a = ex2(a);
-                b = ex2(b);
-                sum = add2(sum, pk2(a, b));
+                if (EMU && e % (EMU + !EMU) == EMU - 1) {
+                    w = ex2_poly<P_SHIFT_T ? 4 : 3>(w);
+                    upk2(w, a, b);
+                } else {
+                    upk2(w, a, b);
+                    a = ex2(a);
+                    b = ex2(b);
+                    w = pk2(a, b);
+                }
+                sum[e & 1] = add2(sum[e & 1], w);
                 if constexpr (SPLIT) split16(a, b, &p[e], &lo[e]);
                 else p[e] = pack16<T>(a, b);
             }
-            tmem_st32(s_addr + e0 / 2, p);
-            if constexpr (SPLIT) tmem_st32(s_addr + 64 + e0 / 2, lo);
+            tmem_st32(s_addr + half * 32, p);
+            if constexpr (SPLIT) tmem_st32(s_addr + 64 + half * 32, lo);
+            if (half == 1 || HALVES) {
+                tmem_st_wait();
+                tc_fence_before();
+                __syncwarp();
+                if ((threadIdx.x & 31) == 0) mbar_arrive(half ? &bars.p_full[buf] : &bars.p_half[buf]);
+            }
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if ((threadIdx.x & 31) == 0) mbar_arrive(&bars.p_full[buf]);
+        ++f.steps[0];
+        if (!last) ++f.parts;
         float a, b;
-        upk2(sum, a, b);
+        upk2(add2(sum[0], sum[1]), a, b);
         l += a + b;
         return true;
     }

@@ -16,17 +16,14 @@ constexpr int TILE_ROWS = 128;
 constexpr int CHUNK = 64;                                // 16-bit values in a 128-byte swizzled row
 constexpr int CHUNK_BYTES = TILE_ROWS * CHUNK * 2;       // [128 rows][64 values]
 
-// ---- shared-memory operands, 128-byte swizzle: 8 rows of 128 bytes are an atom of 1024 bytes
+// ---- shared-memory operands, 128-byte swizzle: 8 rows of 128 bytes are an atom of 1024 bytes. A descriptor's upper half is
+// the same for all of them; the lower half is the address and, for MN-major ones, the way to the next 64 values.
 // K-major (rows of 64 values along the contraction): the atoms of further rows follow at 1024 bytes.
-__device__ __forceinline__ uint64_t desc_k_major(unsigned smem) {
-    return (uint64_t)((smem & 0x3ffff) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
 // MN-major (rows along the contraction, 64 values of the other axis each): eight more rows follow at 1024 bytes, the next
 // 64 values of a row at CHUNK_BYTES.
-__device__ __forceinline__ uint64_t desc_mn_major(unsigned smem) {
-    return (uint64_t)((smem & 0x3ffff) >> 4) | ((uint64_t)(CHUNK_BYTES >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
-}
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k_major(unsigned smem) { return ((smem & 0x3ffff) >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn_major(unsigned smem) { return ((smem & 0x3ffff) >> 4) | ((uint32_t)(CHUNK_BYTES >> 4) << 16); }
 
 // 16-bit operands (both fp16 or both bf16), fp32 accumulator, M = 128
 template <typename T>
@@ -35,18 +32,26 @@ __device__ constexpr uint32_t idesc_f16(int n, bool b_mn_major) {
     return (1u << 4) | (f << 7) | (f << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
-// D[128 x n] (+)= A[128 x 16] B[16 x n], A and B in shared memory
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+// One thread of a converged warp. The instruction takes its operands from the warp's uniform registers: issued from code
+// that all lanes run, they are computed there; from a branch that a single lane took, each had to be moved over first
+// (100 clocks an instruction and more).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+// D[128 x n] (+)= A[128 x 16] B[16 x n], A and B in shared memory (lower halves of their descriptors)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tmov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(DESC_HI)
                  : "memory");
 }
 // the same with A in tensor memory (16-bit pairs, one column per pair)
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tmov.b64 db, {%2, %5};\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "r"(DESC_HI)
                  : "memory");
 }
 // arrives on the barrier once everything this thread has issued to the tensor cores is done
@@ -111,6 +116,41 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// the largest of three; a NaN among numbers is passed over
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
+}
+// 2^x of a pair on the FMA pipe, for x up to 127: x = n + f with n = floor(x) (adding 1.5 2^23 rounded down leaves n in the low
+// mantissa bits), 2^f by the polynomial of degree DEG that has the least relative error on [0, 1] among those that are
+// 1 at 0 (degree 3: 8.6e-5, degree 4: 3.0e-6; a linear programme's solution), times 2^n put together from its bits. x below -127
+// (and -inf) gives exactly 0, NaN gives NaN. Eleven or twelve instructions on pipes that a softmax leaves idle, against
+// two on the special-function unit, which it keeps busiest.
+template <int DEG>
+__device__ __forceinline__ f2 ex2_poly(f2 x) {
+    float a, b;
+    upk2(x, a, b);
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));     // -127
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
+    x = pk2(a, b);
+    const f2 magic = pk2(12582912.0f, 12582912.0f);
+    f2 r;
+    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(magic));
+    const f2 f = sub2(x, sub2(r, magic));
+    f2 y;
+    if constexpr (DEG == 3) {
+        y = fma2(pk2(0.07706713676452637f, 0.07706713676452637f), f, pk2(0.22764486074447632f, 0.22764486074447632f));
+        y = fma2(y, f, pk2(0.6951168179512024f, 0.6951168179512024f));
+    } else {
+        y = fma2(pk2(0.013427390716969967f, 0.013427390716969967f), f, pk2(0.05224123224616051f, 0.05224123224616051f));
+        y = fma2(y, f, pk2(0.24128079414367676f, 0.24128079414367676f));
+        y = fma2(y, f, pk2(0.6930447816848755f, 0.6930447816848755f));
+    }
+    y = fma2(y, f, pk2(1.0f, 1.0f));
+    const uint32_t n0 = ((uint32_t)r << 23) + 0x3f800000u, n1 = ((uint32_t)(r >> 32) << 23) + 0x3f800000u;
+    return mul2(y, pk2(__uint_as_float(n0), __uint_as_float(n1)));
 }
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
