@@ -86,8 +86,9 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
     if (q_stride < (long long)n_q * D || k_stride < (long long)n_kv * D || v_stride < (long long)n_kv * D || q_stride % 8 ||
         k_stride % 8 || v_stride % 8 || !al16(q) || !al16(k) || !al16(v) || !al16(out) || out == q || out == k || out == v)
         return cudaErrorInvalidValue;
-    const int per = prompt_rows(D);
-    const long long n_slots = seq_start ? rows / per + n_seqs : (rows + per - 1) / per, grid = n_slots * n_q;
+    // Two query tiles of a CTA are the same 128 rows of two heads where the group's size is even, else 256 rows of one head
+    const int pair = D < 256 && n_q / n_kv % 2 == 0, per = D == 256 || pair ? TILE_ROWS : 2 * TILE_ROWS;
+    const long long n_slots = seq_start ? rows / per + n_seqs : (rows + per - 1) / per, grid = n_slots * (pair ? n_q / 2 : n_q);
     if (grid > INT_MAX) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
     CUtensorMap mq, mk, mv;
@@ -98,10 +99,11 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
 #define TILES(D_)                                                                                                            \
     do {                                                                                                                     \
         using Ti = PromptTiles<D_, T>;                                                                                       \
-        st = allow_smem(k_attn_prompt<D_, T>, Ti::SMEM);                                                                     \
+        constexpr int SMEM = Ti::SMEM + PROMPT_OUT<D_>;                                                                      \
+        st = allow_smem(k_attn_prompt<D_, T>, SMEM);                                                                         \
         if (st != cudaSuccess) return st;                                                                                    \
-        launch_pdl((k_attn_prompt<D_, T>), (unsigned)grid, Ti::WARPS * 32, Ti::SMEM, stream, mq, mk, mv, q, k, v, out, seq_start, \
-                   n_seqs, (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E, (int)n_slots);           \
+        launch_pdl((k_attn_prompt<D_, T>), (unsigned)grid, Ti::WARPS * 32, SMEM, stream, mq, mk, mv, q, k, v, out, seq_start, n_seqs, \
+                   (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E, (int)n_slots, pair);             \
     } while (0)
     if (D == 64) TILES(64); else if (D == 128) TILES(128); else TILES(256);
 #undef TILES

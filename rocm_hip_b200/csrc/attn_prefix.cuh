@@ -149,13 +149,13 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
         for (int j = 0; j < tiles_i; ++j) {
             const unsigned seen = __ballot_sync(0xffffffffu, next);
             next = look(j + 1);
-            uint32_t x[128];
-            if (!Ti::scores(bars, i, f, x)) break;
-            if (seen != 0xffffffffu)
+            if (!Ti::softmax_step(bars, i, j == 0, j + 1 == tiles_i, f, c_row, m, l, [&](uint32_t (&x)[128]) {
+                    if (seen != 0xffffffffu)
 #pragma unroll
-                for (int e = 0; e < 128; ++e)
-                    if (!(seen >> (e / 4) & 1)) x[e] = 0xff800000u;
-            if (!Ti::weights(bars, i, j == 0, j + 1 == tiles_i, f, x, c_row, m, l)) break;
+                        for (int e = 0; e < 128; ++e)
+                            if (!(seen >> (e / 4) & 1)) x[e] = 0xff800000u;
+                }))
+                break;
         }
         if (tiles_i > 0 && warp_wait(&bars.o_full[i], 0, &bars.dead)) {
             tc_fence_after();

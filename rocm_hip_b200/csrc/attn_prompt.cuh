@@ -11,12 +11,17 @@
 
 namespace b200 {
 
-// Two query tiles per CTA, one for the 256-wide heads; K and V stages as large as shared memory allows beside them
+// Two query tiles per CTA, one for the 256-wide heads; K and V stages as large as shared memory allows beside them. The 64-wide
+// heads leave room for a buffer through which finished rows leave (2 KB a warp), so that the next query tile can come as
+// soon as the last scores against the old one are done (61 sequences of 200 rows: 82 -> 69 us); the others send their rows
+// out through the query tile's memory (a buffer in the place of a ring stage cost 2 % of long prompts).
 template <int D, typename T>
 using PromptTiles = Tiles<D, D == 256 ? 1 : 2, D < 128 ? D : 128, D == 64 ? 8 : 5, false, T>;
-__host__ __device__ constexpr int prompt_rows(int D) { return D == 256 ? TILE_ROWS : 2 * TILE_ROWS; }   // query rows of a CTA
+template <int D>
+constexpr int PROMPT_OUT = D == 64 ? 8 * 2048 : 0;
 
-// What a CTA works on next: up to ROWS query rows of one head of one sequence
+// What a CTA works on next: one or two query tiles of a sequence. Two are the same rows of two heads that share a key head
+// (pair: the group has an even number of heads; both tiles then see the same keys), or 256 rows of one head.
 struct PromptItem {
     int h, first, q0, end;      // head; the sequence's first row; the first query row; the sequence's end
     int n[2];                   // key tiles per query tile; n[0] == 0: there is nothing more
@@ -49,15 +54,17 @@ __device__ __forceinline__ int block_answer(PromptBars& pb) {   // the block's i
 // The grid is all blocks of work, heaviest first as far as one pass over the batch knows; a CTA that has finished one takes
 // the next that nobody has begun. Its roles run ahead of one another: while the softmax warps still write one block's rows,
 // the schedule warp has looked up the next block, its first K and V tiles are on their way, and the tensor cores begin as
-// soon as the query tile's memory is free. (One CTA per block: 61 sequences of 200 rows, 16 heads of 64, took 98 us, most of
+// soon as the last scores against the query tile are done. (One CTA per block: 61 sequences of 200 rows, 16 heads of 64, took 98 us, most of
 // it the way from a CTA's start to its first product and from its last to its end.)
 template <int D, typename T>
 __global__ void __launch_bounds__(PromptTiles<D, T>::WARPS * 32, 1)
 k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
               const T* q, const T* k, const T* v, T* out, const int* seq_start, int n_seqs, int rows, int n_q, int G,
-              long long q_stride, long long k_stride, long long v_stride, float scale2, int n_slots) {
+              long long q_stride, long long k_stride, long long v_stride, float scale2, int n_slots, int pair) {
     using Ti = PromptTiles<D, T>;
-    constexpr int NQ = D == 256 ? 1 : 2, SC = D < 128 ? D : 128, ROWS = prompt_rows(D);
+    constexpr int NQ = D == 256 ? 1 : 2, SC = D < 128 ? D : 128;
+    const int ROWS = NQ == 2 && !pair ? 2 * TILE_ROWS : TILE_ROWS, n_heads = pair ? n_q / 2 : n_q;   // rows and heads of a block
+    const int dh = pair ? 1 : 0, dq = pair ? 0 : TILE_ROWS;          // from the first query tile to the second
     extern __shared__ unsigned char smem_raw[];
     __shared__ TileBars bars;
     __shared__ PromptBars pb;
@@ -71,7 +78,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         for (int i = 0; i < 2; ++i) {
             mbar_init(&pb.item_full[i], 1);
             mbar_init(&pb.item_empty[i], NQ * 4 + 2);
-            mbar_init(&pb.q_empty[i], 4);
+            mbar_init(&pb.q_empty[i], PROMPT_OUT<D> ? 1 : 4);
         }
         mbar_init(&pb.asked, 1);
         mbar_fence_init();
@@ -104,7 +111,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 // slot s of the packed batch is tile s - f(b) of sequence b, f(b) = floor(start(b) / ROWS) + b, the last b with
                 // f(b) <= s; f(b + 1) - f(b) is at least the number of tiles b has. Slots are taken from the last one down, so
                 // that in a sequence the tiles with the most keys come first.
-                const int slot = n_slots - 1 - block / n_q;
+                const int slot = n_slots - 1 - block / n_heads;
                 int first = 0, end = rows, tile = slot;
                 if (seq_start) {
                     int lo = 0, hi = n_seqs;            // the last b with f(b) <= slot is in [lo - 1, hi): 32 probes a step
@@ -124,13 +131,13 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                     tile = slot - (first / ROWS + b);
                 }
                 if (tile >= 0 && tile <= (end - first) / ROWS && first + tile * ROWS < end) {   // (no overflow on bad borders)
-                    it.h = block % n_q;
+                    it.h = block % n_heads << dh;
                     it.first = first;
                     it.q0 = first + tile * ROWS;
                     it.end = end;
 #pragma unroll
                     for (int i = 0; i < NQ; ++i) {      // those up to the last row's own place
-                        const int a = it.q0 + i * TILE_ROWS;
+                        const int a = it.q0 + i * dq;
                         it.n[i] = a < end ? (min(a + TILE_ROWS, end) - 1 - first) / TILE_ROWS + 1 : 0;
                     }
                 }
@@ -173,7 +180,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 if (lane == 0) mbar_expect(&bars.q_full[i], Ti::QTILE);
                 __syncwarp();
                 if (lane < D / CHUNK)
-                    tma_3d(smem + i * Ti::QTILE + lane * CHUNK_BYTES, &mq, lane * CHUNK, it.h, it.q0 + i * TILE_ROWS, &bars.q_full[i]);
+                    tma_3d(smem + i * Ti::QTILE + lane * CHUNK_BYTES, &mq, lane * CHUNK, it.h + i * dh, it.q0 + i * dq, &bars.q_full[i]);
             }
             for (int j = 0; j < n_all; ++j) {
                 if (j + 1 < n_all) put(&mk, j + 1);
@@ -185,7 +192,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         TileFlow f;
         PromptItem it;
         while (next_item(&it))
-            if (!Ti::products(bars, smem, ring, it.n[0], it.n[1], f)) break;
+            if (!Ti::products(bars, smem, ring, it.n[0], it.n[1], f, PROMPT_OUT<D> ? pb.q_empty : nullptr)) break;
     } else if (warp < NQ * 4) {
         Ti::many_registers();
         // ---- softmax: thread = row
@@ -193,61 +200,67 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         TileFlow f;
         PromptItem it;
         while (next_item(&it)) {
-            const int tiles = i ? it.n[1] : it.n[0], h = it.h, first = it.first, end = it.end, t0 = it.q0 + i * TILE_ROWS, row = t0 + r;
+            const int tiles = i ? it.n[1] : it.n[0], h = it.h + i * dh, first = it.first, end = it.end, t0 = it.q0 + i * dq, row = t0 + r;
             if (tiles == 0) continue;
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
             for (int j = 0; j < tiles && ok; ++j) {
-                uint32_t x[128];
-                ok = Ti::scores(bars, i, f, x);
-                if (!ok) break;
-                const int last = row - first - j * TILE_ROWS;   // the last key of this tile that the row sees
-                if (j + 1 == tiles)   // (uniform) only a query tile's last key tile reaches past any of its rows
+                const int seen = row - first - j * TILE_ROWS;   // the last key of this tile that the row sees
+                ok = Ti::softmax_step(bars, i, j == 0, j + 1 == tiles, f, scale2, m, l, [&](uint32_t (&x)[128]) {
+                    if (j + 1 == tiles)   // (uniform) only a query tile's last key tile reaches past any of its rows
 #pragma unroll
-                    for (int c = 0; c < 128; ++c)
-                        if (c > last) x[c] = 0xff800000u;
-                ok = Ti::weights(bars, i, j == 0, j + 1 == tiles, f, x, scale2, m, l);
+                        for (int e = 0; e < 128; ++e)
+                            if (e > seen) x[e] = 0xff800000u;
+                });
             }
             if (!ok || !warp_wait(&bars.o_full[i], f.items[0] & 1, &bars.dead)) break;
             ++f.items[0];
             tc_fence_after();
-            // O / l through the Q tile's shared memory (its last S is done), so that whole rows leave the warp together
+            // O / l through shared memory, CW columns at a time, so that the rows' stretches leave the warp together
+            constexpr bool BUF = PROMPT_OUT<D> > 0;
+            constexpr int CW = BUF ? 32 : D, UNITS = CW / 8;
             const uint32_t o_addr = bars.tmem + 256 + i * D + ((uint32_t)(threadIdx.x & 96) << 16);
-            unsigned char* mine = smem + (i * TILE_ROWS + (warp & 3) * 32) * (D * 2);
+            unsigned char* mine = BUF ? ring + Ti::RING + warp * 2048 : smem + (i * TILE_ROWS + (warp & 3) * 32) * (D * 2);
             const float inv = 1.0f / l;
             bool bad = false;
-            for (int c = 0; c < D; c += 32) {
-                uint32_t o[32];
-                tmem_ld32(o_addr + c, o);
-                tmem_ld_wait();
-                tmem_pin(o);
+            for (int c0 = 0; c0 < D; c0 += CW) {
+                for (int c = 0; c < CW; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + c0 + c, o);
+                    tmem_ld_wait();
+                    tmem_pin(o);
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    float y[8];
+                    for (int e = 0; e < 32; e += 8) {
+                        float y[8];
 #pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        y[t] = __uint_as_float(o[e + t]) * inv;
-                        bad |= !(fabsf(y[t]) < INFINITY);
+                        for (int t = 0; t < 8; ++t) {
+                            y[t] = __uint_as_float(o[e + t]) * inv;
+                            bad |= !(fabsf(y[t]) < INFINITY);
+                        }
+                        // (units of 16 bytes, stirred so that neither eight lanes' rows nor eight units share a bank)
+                        const int u = (c + e) / 8, at = BUF ? u ^ (lane >> 1 & 3) : u ^ (lane & 7);
+                        *reinterpret_cast<uint4*>(mine + lane * (CW * 2) + at * 16) = Io<T>::pack(y);
                     }
-                    const int u = (c + e) / 8;
-                    *reinterpret_cast<uint4*>(mine + lane * (D * 2) + ((u ^ (lane & 7)) * 16)) = Io<T>::pack(y);
                 }
-            }
-            __syncwarp();
-            constexpr int UNITS = D / 8;
+                __syncwarp();
 #pragma unroll 4
-            for (int e = lane; e < 32 * UNITS; e += 32) {
-                const int rr = e / UNITS, u = e % UNITS, t = t0 + (warp & 3) * 32 + rr;
-                const uint4 y = *reinterpret_cast<const uint4*>(mine + rr * (D * 2) + ((u ^ (rr & 7)) * 16));
-                if (t < end) st_stream(reinterpret_cast<unsigned char*>(out + ((long long)t * n_q + h) * D) + u * 16, y);
+                for (int e = lane; e < 32 * UNITS; e += 32) {
+                    const int rr = e / UNITS, u = e % UNITS, t = t0 + (warp & 3) * 32 + rr;
+                    const int at = BUF ? u ^ (rr >> 1 & 3) : u ^ (rr & 7);
+                    const uint4 y = *reinterpret_cast<const uint4*>(mine + rr * (CW * 2) + at * 16);
+                    if (t < end) st_stream(reinterpret_cast<unsigned char*>(out + ((long long)t * n_q + h) * D + c0) + u * 16, y);
+                }
+                __syncwarp();
             }
-            // the query tile's memory may take the next one
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pb.q_empty[i]);
+            if (!BUF) {   // the query tile's memory may take the next one
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pb.q_empty[i]);
+            }
             // A weight of 0 times a non-finite v is not 0 on the tensor cores: rows that came out non-finite are computed again
             // from the keys they may see alone
             unsigned again = __ballot_sync(0xffffffffu, bad && row < end);
+            __syncwarp();
             while (again) {
                 const int t = t0 + (warp & 3) * 32 + __ffs(again) - 1;
                 again &= again - 1;

@@ -62,7 +62,8 @@ struct Tiles {
     static constexpr int PARTS = D / SC;
     static constexpr int QTILE = TILE_ROWS * D * 2;                        // one query tile, one half of a split one
     static constexpr int Q_BYTES = NQ * QTILE * (SPLIT ? 2 : 1);           // [NQ][hi, lo][D / 64][128 rows][64 values]
-    static constexpr int SMEM = 1024 + Q_BYTES + ST * STAGE;
+    static constexpr int RING = ST * STAGE;
+    static constexpr int SMEM = 1024 + Q_BYTES + RING;
     static constexpr int WARPS = NQ == 2 ? 12 : 7;                         // softmax, tensor cores, copies, schedule (and an idle one)
     // NQ = 2: the products of a tile's first half of the keys begin while the second half is still in the softmax (8,192 rows,
     // 32 heads of 128: 1,246 -> 1,295 TFLOP/s). With one query tile the next S fills that time (heads of 256: 1,286 without,
@@ -70,14 +71,14 @@ struct Tiles {
     static constexpr bool HALVES = NQ == 2;
     static constexpr int P_SHIFT_T = std::is_same<T, __half>::value ? 7 : 0;   // fp16 weights are held times 2^7 (at most 2^15)
 
-    // A softmax thread holds its row's 128 scores: 208 registers. Twelve warps start with 168 each (64,512 in all); the four
-    // that compute nothing go down to 80 and the eight softmax warps up, 4 x 32 x 80 + 8 x 32 x 208 = 63,488. (Six warps
+    // A softmax thread holds its row's 128 scores: 224 registers. Twelve warps start with 168 each (64,512 in all); the four
+    // that compute nothing go down to 56 and the eight softmax warps up, 4 x 32 x 56 + 8 x 32 x 224 = 64,512. (Six warps
     // may have 255 from the start.)
     static __device__ __forceinline__ void few_registers() {
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     }
     static __device__ __forceinline__ void many_registers() {
-        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+        if constexpr (NQ == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
     }
 
     // Barriers and tensor memory; all threads. q_arrivals: how many fill a query tile.
@@ -138,9 +139,9 @@ struct Tiles {
     static __device__ __forceinline__ unsigned parity(unsigned steps) { return NQ == 1 ? steps >> 1 & 1 : steps & 1; }
 
     // One warp: everything the tensor cores do for n0 / n1 key tiles of the query tiles. The ring brings
-    // K 0, K 1, V 0, K 2, V 1, ...  False: given up.
+    // K 0, K 1, V 0, K 2, V 1, ...  q_empty: told when a query tile's last scores are done. False: given up.
     static __device__ __forceinline__ bool products(TileBars& bars, const unsigned char* qs, const unsigned char* ring, int n0, int n1,
-                                                    TileFlow& f) {
+                                                    TileFlow& f, unsigned long long* q_empty = nullptr) {
         constexpr uint32_t id_s = idesc_f16<T>(TILE_ROWS, false), id_o = idesc_f16<T>(SC, true);
         constexpr int Z = SPLIT ? 2 : 1;
         const uint32_t tmem = bars.tmem, q_desc = desc_k_major(smem_u32(qs)), k_desc = desc_k_major(smem_u32(ring)),
@@ -201,6 +202,7 @@ struct Tiles {
             if (dead) return false;
             tc_fence_after();
             score(i, buffer(f.steps[i], i), ks);
+            if (q_empty && (i ? n1 : n0) == 1 && elect_one()) mma_commit(&q_empty[i]);
         }
         give(ks);
         for (int j = 0; j < n_all; ++j) {
@@ -209,6 +211,7 @@ struct Tiles {
             if (dead) return false;
             if (NQ == 1 && more) {
                 score(0, buffer(f.steps[0] + 1, 0), ks);
+                if (q_empty && j + 2 == n_all && elect_one()) mma_commit(&q_empty[0]);
                 give(ks);
             }
             vs = take();
@@ -230,7 +233,10 @@ struct Tiles {
                 if (NQ == 1 || j + 1 == ni) {
                     if (elect_one()) mma_commit(j + 1 == ni ? &bars.o_full[i] : &bars.o_part);
                 }
-                if (NQ == 2 && j + 1 < ni) score(i, i, ks);
+                if (NQ == 2 && j + 1 < ni) {
+                    score(i, i, ks);
+                    if (q_empty && j + 2 == ni && elect_one()) mma_commit(&q_empty[i]);
+                }
             }
             if (NQ == 2 && more) give(ks);
             give(vs);
@@ -240,81 +246,90 @@ struct Tiles {
         return true;
     }
 
-    // A softmax thread: its row's scores against the next key tile into x, once they are there
-    static __device__ __forceinline__ bool scores(TileBars& bars, int i, const TileFlow& f, uint32_t (&x)[128]) {
-        const int buf = buffer(f.steps[0], i);
-        if (!warp_wait(&bars.s_full[buf], parity(f.steps[0]), &bars.dead)) return false;
-        tc_fence_after();
-        const uint32_t s_addr = bars.tmem + buf * 128 + ((uint32_t)(threadIdx.x & 96) << 16);
+    // 64 scores of a row (columns 64 half ..) into weights: 16-bit pairs p (and lo, SPLIT), their sum added to `sum`.
+    // Of every EMU pairs one takes the polynomial: the special-function unit gives 16 values a clock and SM, two query tiles
+    // of 128-wide heads want 128 x 128 of them every 1,024 clocks, which is all of them (8,192 rows, 32 heads, EMU 0, 3, 4, 6:
+    // 1,242, 1,272, 1,295 and 1,290 TFLOP/s), narrower heads more (64: 660, 731, 719 with 0, 3, 4); 256-wide heads half of
+    // them, and the polynomial's instructions only cost (1,325, 1,249, 1,286 with 0, 3, 4).
+    static constexpr int EMU = SPLIT || NQ == 1 ? 0 : D == 64 ? 3 : 4;
+    static __device__ __forceinline__ void exps(const uint32_t (&x)[128], int half, f2 c2, f2 neg2, uint32_t (&p)[32],
+                                                uint32_t (&lo)[SPLIT ? 32 : 1], f2 (&sum)[2]) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + c * 32, x + c * 32);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_pin(x + c * 32);
-        return true;
+        for (int e = 0; e < 32; ++e) {
+            const int at = half * 64 + 2 * e;
+            f2 w = fma2(pk2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), c2, neg2);
+            float a, b;
+            if (EMU && e % (EMU + !EMU) == EMU - 1) {
+                w = ex2_poly<P_SHIFT_T ? 4 : 3>(w);
+                upk2(w, a, b);
+            } else {
+                upk2(w, a, b);
+                a = ex2(a);
+                b = ex2(b);
+                w = pk2(a, b);
+            }
+            sum[e & 1] = add2(sum[e & 1], w);
+            if constexpr (SPLIT) split16(a, b, &p[e], &lo[e]);
+            else p[e] = pack16<T>(a, b);
+        }
     }
-
-    // ... and, masked scores (-inf) in x, from there to P in tensor memory; c > 0 turns scores into powers of two. first / last: of
-    // the query tile's key tiles. (f.steps[0] counts this role's steps whichever query tile it has.)
-    static __device__ __forceinline__ bool weights(TileBars& bars, int i, bool first, bool last, TileFlow& f, uint32_t (&x)[128], float c,
-                                                   float& m, float& l) {
-        const int buf = buffer(f.steps[0], i);
-        const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
-        const uint32_t s_addr = bars.tmem + buf * 128 + lanes, o_addr = bars.tmem + 256 + i * D + lanes;
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};     // four chains of three-way maxima
+    static __device__ __forceinline__ float row_max(const uint32_t (&x)[128]) {   // four chains of three-way maxima
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < 128; e += 8)
 #pragma unroll
             for (int t = 0; t < 4; ++t) top[t] = max3(top[t], __uint_as_float(x[e + 2 * t]), __uint_as_float(x[e + 2 * t + 1]));
-        const float mx = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+        return fmaxf(max3(top[0], top[1], top[2]), top[3]);
+    }
+
+    // A softmax thread's part of one key tile: the row's scores, once they are there, masked (hide(x) sets what the row does not
+    // see to -inf), turned into weights in tensor memory; c > 0 turns scores into powers of two; first / last: of the query
+    // tile's key tiles. (f.steps[0] counts this role's steps whichever query tile it has.) False: given up.
+    // (The first half's weights computed with the maximum so far, while the tile's own is still being found, and again in the
+    // rare tile where it has grown by 2^8: 1,197 against 1,270 TFLOP/s for 8,192 rows, 32 heads of 128. The special-function
+    // unit is what the two query tiles' warps share, and there is nothing to gain from being at it earlier.)
+    template <typename Hide>
+    static __device__ __forceinline__ bool softmax_step(TileBars& bars, int i, bool first, bool last, TileFlow& f, float c, float& m,
+                                                        float& l, Hide hide) {
+        const int buf = buffer(f.steps[0], i);
+        if (!warp_wait(&bars.s_full[buf], parity(f.steps[0]), &bars.dead)) return false;
+        tc_fence_after();
+        const uint32_t lanes = (uint32_t)(threadIdx.x & 96) << 16;
+        const uint32_t s_addr = bars.tmem + buf * 128 + lanes, o_addr = bars.tmem + 256 + i * D + lanes;
+        uint32_t x[128];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tmem_ld32(s_addr + e * 32, x + e * 32);
+        tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tmem_pin(x + e * 32);
+        hide(x);
+        const float mx = row_max(x);
         if (first) m = mx;
         else if (__any_sync(0xffffffffu, (mx - m) * c > 8.0f)) {
             // O holds the tiles before this one. NQ = 2: their products were issued before this S, so they are done. NQ = 1:
             // the last of them comes behind this S.
             if (NQ == 1 && !warp_wait(&bars.o_part, (f.parts - 1) & 1, &bars.dead)) return false;
             tc_fence_after();
-            const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.0f : ex2((m - mn) * c);
+            const float mn = fmaxf(m, mx), k = mn == -INFINITY ? 1.0f : ex2((m - mn) * c);
             m = mn;
-            l *= f;
+            l *= k;
             for (int e0 = 0; e0 < D; e0 += 32) {
                 uint32_t o[32];
                 tmem_ld32(o_addr + e0, o);
                 tmem_ld_wait();
                 tmem_pin(o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * k);
                 tmem_st32(o_addr + e0, o);
             }
         }
         const float neg = m == -INFINITY ? 0.0f : P_SHIFT_T - m * c;
         const f2 neg2 = pk2(neg, neg), c2 = pk2(c, c);
-        // Of every EMU pairs one takes the polynomial: the special-function unit gives 16 values a clock and SM, two query tiles
-        // of 128-wide heads want 128 x 128 of them every 1,024 clocks, which is all of them (0, 3, 4, 6: 1,242, 1,272, 1,295 and
-        // 1,290 TFLOP/s), narrower heads more (64: 660, 731, 719 with 0, 3, 4); 256-wide heads half of them, and the
-        // polynomial's instructions only cost (1,325, 1,249, 1,286 with 0, 3, 4).
-        constexpr int EMU = SPLIT || NQ == 1 ? 0 : D == 64 ? 3 : 4;
         f2 sum[2] = {pk2(0.0f, 0.0f), pk2(0.0f, 0.0f)};
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
             uint32_t p[32], lo[SPLIT ? 32 : 1];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                const int at = half * 64 + 2 * e;
-                f2 w = fma2(pk2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), c2, neg2);
-                float a, b;
-                if (EMU && e % (EMU + !EMU) == EMU - 1) {
-                    w = ex2_poly<P_SHIFT_T ? 4 : 3>(w);
-                    upk2(w, a, b);
-                } else {
-                    upk2(w, a, b);
-                    a = ex2(a);
-                    b = ex2(b);
-                    w = pk2(a, b);
-                }
-                sum[e & 1] = add2(sum[e & 1], w);
-                if constexpr (SPLIT) split16(a, b, &p[e], &lo[e]);
-                else p[e] = pack16<T>(a, b);
-            }
+            exps(x, half, c2, neg2, p, lo, sum);
             tmem_st32(s_addr + half * 32, p);
             if constexpr (SPLIT) tmem_st32(s_addr + 64 + half * 32, lo);
             if (half == 1 || HALVES) {
