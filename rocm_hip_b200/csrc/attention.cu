@@ -65,10 +65,18 @@ bool row_map(CUtensorMap* m, const T* p, int D, int heads, long long rows, long 
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Lets the kernel have `bytes` of dynamic shared memory on the current device
+// Lets a kernel have `bytes` of dynamic shared memory on the current device: asked once per kernel and device (`done`: a
+// bit per device, the caller's static for that kernel), for the call costs as much as a launch
 template <typename K>
-cudaError_t allow_smem(K kernel, int bytes) {
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+cudaError_t allow_smem(K kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int dev = 0;
+    cudaError_t st = cudaGetDevice(&dev);
+    if (st != cudaSuccess) return st;
+    const unsigned long long bit = dev < 64 ? 1ull << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    st = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (st == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return st;
 }
 
 // ---------------------------------------------------------------- prompts
@@ -86,9 +94,16 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
     if (q_stride < (long long)n_q * D || k_stride < (long long)n_kv * D || v_stride < (long long)n_kv * D || q_stride % 8 ||
         k_stride % 8 || v_stride % 8 || !al16(q) || !al16(k) || !al16(v) || !al16(out) || out == q || out == k || out == v)
         return cudaErrorInvalidValue;
-    // Two query tiles of a CTA are the same 128 rows of two heads where the group's size is even, else 256 rows of one head
-    const int pair = D < 256 && n_q / n_kv % 2 == 0, per = D == 256 || pair ? TILE_ROWS : 2 * TILE_ROWS;
-    const long long n_slots = seq_start ? rows / per + n_seqs : (rows + per - 1) / per, grid = n_slots * (pair ? n_q / 2 : n_q);
+    // How a CTA's two query tiles come about (attn_prompt.cuh): two heads of an even group, else 256 rows; and, where those
+    // are fewer blocks than SMs, one tile whose keys are shared between the two: half the steps for the block that takes
+    // longest, for twice the K and V bytes a step (one sequence of 512 and 1,024 rows, 16 / 8 heads of 128: 12.8 -> 10.1 and
+    // 19.1 -> 14.4 us; at 152 blocks, 2,427 rows, 40.3 -> 40.0 in bf16 and 40.4 -> 50.9 in fp16)
+    const int slots128 = (int)(seq_start ? rows / TILE_ROWS + n_seqs : (rows + TILE_ROWS - 1) / TILE_ROWS);
+    const long long slots256 = seq_start ? rows / (2 * TILE_ROWS) + n_seqs : (rows + 2 * TILE_ROWS - 1) / (2 * TILE_ROWS);
+    const bool even = n_q / n_kv % 2 == 0;
+    int mode = D == 256 ? BY_ROWS : even ? BY_HEADS : BY_ROWS;
+    if (D < 256 && (even ? (long long)slots128 * (n_q / 2) : slots256 * n_q) < sm_count()) mode = BY_KEYS;
+    const long long n_slots = D < 256 && mode == BY_ROWS ? slots256 : slots128, grid = n_slots * (mode == BY_HEADS ? n_q / 2 : n_q);
     if (grid > INT_MAX) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
     CUtensorMap mq, mk, mv;
@@ -96,16 +111,22 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
         !row_map<T>(&mv, v, D, n_kv, rows, v_stride))
         return cudaErrorInvalidValue;
     cudaError_t st;
-#define TILES(D_)                                                                                                            \
+#define TILES(D_, MODE_)                                                                                                     \
     do {                                                                                                                     \
         using Ti = PromptTiles<D_, T>;                                                                                       \
         constexpr int SMEM = Ti::SMEM + PROMPT_OUT<D_>;                                                                      \
-        st = allow_smem(k_attn_prompt<D_, T>, SMEM);                                                                         \
+        static std::atomic<unsigned long long> done;                                                                         \
+        st = allow_smem(k_attn_prompt<D_, T, MODE_>, SMEM, done);                                                                  \
         if (st != cudaSuccess) return st;                                                                                    \
-        launch_pdl((k_attn_prompt<D_, T>), (unsigned)grid, Ti::WARPS * 32, SMEM, stream, mq, mk, mv, q, k, v, out, seq_start, n_seqs, \
-                   (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E, (int)n_slots, pair);             \
+        launch_pdl((k_attn_prompt<D_, T, MODE_>), (unsigned)grid, Ti::WARPS * 32, SMEM, stream, mq, mk, mv, q, k, v, out, seq_start, \
+                   n_seqs, (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E, (int)n_slots);           \
     } while (0)
-    if (D == 64) TILES(64); else if (D == 128) TILES(128); else TILES(256);
+#define MODES(D_)                                                                                                            \
+    do {                                                                                                                     \
+        if (mode == BY_KEYS) TILES(D_, BY_KEYS); else if (mode == BY_HEADS) TILES(D_, BY_HEADS); else TILES(D_, BY_ROWS);    \
+    } while (0)
+    if (D == 64) MODES(64); else if (D == 128) MODES(128); else TILES(256, BY_ROWS);
+#undef MODES
 #undef TILES
     return launched();
 }
@@ -186,7 +207,8 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
     cudaError_t st;
 #define OWN(BOX_)                                                                                                            \
     do {                                                                                                                     \
-        if ((st = allow_smem(k_attn_own<D, T, BOX_>, OwnShape<D>::SMEM)) != cudaSuccess) return st;                          \
+        static std::atomic<unsigned long long> done;                                                                         \
+        if ((st = allow_smem(k_attn_own<D, T, BOX_>, OwnShape<D>::SMEM, done)) != cudaSuccess) return st;                         \
         launch_pdl((k_attn_own<D, T, BOX_>), (unsigned)pl.grid_own, OwnShape<D>::WARPS * 32, OwnShape<D>::SMEM, stream, ok, ov, q, kv, \
                    sc, n_q, n_kv, B, behind, scale2, 2);                                                                     \
     } while (0)
@@ -198,7 +220,8 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
 #define PREFIX(NQ_)                                                                                                       \
     do {                                                                                                                  \
         using Ti = typename PrefixShape<D, NQ_, SPLIT>::Ti;                                                               \
-        if ((st = allow_smem(k_attn_prefix<D, NQ_, T>, Ti::SMEM)) != cudaSuccess) return st;                              \
+        static std::atomic<unsigned long long> done;                                                                      \
+        if ((st = allow_smem(k_attn_prefix<D, NQ_, T>, Ti::SMEM, done)) != cudaSuccess) return st;                             \
         launch_pdl((k_attn_prefix<D, NQ_, T>), grid, Ti::WARPS * 32, Ti::SMEM, stream, mk, mv, q, kv, px, n_q, n_kv, B, prefix, scale2, \
                    pl.row_tiles);                                                                                         \
     } while (0)
@@ -236,6 +259,10 @@ cudaError_t launch_decode(const T* q, const uint16_t* K, const uint16_t* V, int 
 
 // ---------------------------------------------------------------- pages
 
+#ifndef COPY_PER_SM
+#define COPY_PER_SM 8
+#endif
+
 bool good_pages(const b200_kv_pages* kv) {
     return kv && kv->table && kv->lens && kv->refs && kv->info && kv->work && kv->pool && kv->n_seqs > 0 && kv->max_pages > 0 &&
            kv->n_pages > 0 && kv->page_shift >= 0 && kv->page_shift <= 30 &&
@@ -244,16 +271,20 @@ bool good_pages(const b200_kv_pages* kv) {
            kv->part_stride % 16 == 0 && al16(kv->pool) && (long long)kv->n_seqs * kv->max_pages <= (1LL << 40);
 }
 
-// The control kernel as one cluster, then the copies it listed
-template <typename... KA, typename... A>
+// How many CTAs the control kernel takes: one where its tables are small, so that the passes over them are separated by a
+// CTA's barrier only, else a cluster of eight
+bool small_pages(const b200_kv_pages* kv) { return (long long)kv->n_seqs * kv->max_pages <= 16384 && kv->n_pages <= 16384; }
+
+// The control kernel, then the copies it listed
+template <int CTAS, typename... KA, typename... A>
 cudaError_t launch_pages(const b200_kv_pages* kv, cudaStream_t stream, void (*kernel)(KA...), A... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(KVP_CTAS, 1, 1);
+    cfg.gridDim = dim3(CTAS, 1, 1);
     cfg.blockDim = dim3(KVP_THREADS, 1, 1);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = KVP_CTAS;
+    attr[0].val.clusterDim.x = CTAS;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -262,7 +293,7 @@ cudaError_t launch_pages(const b200_kv_pages* kv, cudaStream_t stream, void (*ke
     (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<KA>(args)...);
     const cudaError_t st = launched();
     if (st != cudaSuccess) return st;
-    launch_pdl(k_kv_pages_copy, (unsigned)resident_ctas(256), 256, 0, stream, *kv);
+    launch_pdl(k_kv_pages_copy, (unsigned)(sm_count() * COPY_PER_SM), 256, 0, stream, *kv);
     return launched();
 }
 
@@ -321,19 +352,22 @@ size_t gpu_kv_pages_work_ints(int n_seqs, int n_pages) {
 cudaError_t gpu_kv_pages_fork(const b200_kv_pages* kv, const int* parent, cudaStream_t stream) {
     if (!good_pages(kv) || !parent || parent == kv->lens) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
-    return launch_pages(kv, stream, k_kv_pages_fork, *kv, parent);
+    return small_pages(kv) ? launch_pages<1>(kv, stream, k_kv_pages_fork<1>, *kv, parent)
+                           : launch_pages<8>(kv, stream, k_kv_pages_fork<8>, *kv, parent);
 }
 
 cudaError_t gpu_kv_pages_resize(const b200_kv_pages* kv, const int* new_lens, int* slots, int n_slots, cudaStream_t stream) {
     if (!good_pages(kv) || !new_lens || new_lens == kv->lens || n_slots < 0) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
-    return launch_pages(kv, stream, k_kv_pages_resize, *kv, new_lens, slots, n_slots);
+    return small_pages(kv) ? launch_pages<1>(kv, stream, k_kv_pages_resize<1>, *kv, new_lens, slots, n_slots)
+                           : launch_pages<8>(kv, stream, k_kv_pages_resize<8>, *kv, new_lens, slots, n_slots);
 }
 
 cudaError_t gpu_kv_pages_compact(const b200_kv_pages* kv, cudaStream_t stream) {
     if (!good_pages(kv)) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
-    return launch_pages(kv, stream, k_kv_pages_compact, *kv);
+    return small_pages(kv) ? launch_pages<1>(kv, stream, k_kv_pages_compact<1>, *kv)
+                           : launch_pages<8>(kv, stream, k_kv_pages_compact<8>, *kv);
 }
 
 }  // extern "C"

@@ -143,11 +143,12 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
         *total = all;
         return base + x - v;
     };
-    int total = 0;
+    int total = 0, n_mine = 0, before_mine = 0;      // (of the last round: the only one while B <= NT)
     for (int b0 = 0; b0 < B; b0 += NT) {
         int t;
-        const int before = cta_scan(tiles_of(b0 + tid), &t);
-        if (blockIdx.x == 0 && b0 + tid < B) sc.first[b0 + tid] = total + before;
+        n_mine = tiles_of(b0 + tid);
+        before_mine = total + cta_scan(n_mine, &t);
+        if (blockIdx.x == 0 && b0 + tid < B) sc.first[b0 + tid] = before_mine;
         total += t;
     }
     if (blockIdx.x == 0 && tid == 0) sc.first[B] = total;
@@ -158,15 +159,22 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
     const long long t_end = min(t0 + per, all);
     if (t0 >= t_end) return;
     if (tid == 0) at[0] = B;
-    int done = 0;
-    for (int b0 = 0; b0 < B; b0 += NT) {
-        int t;
-        const int n = tiles_of(b0 + tid), before = done + cta_scan(n, &t);
+    __syncthreads();
+    const auto look = [&](int b, int n, int before) {
         if (n > 0 && t0 >= (long long)before * pl.groups && t0 < (long long)(before + n) * pl.groups) {
-            at[0] = b0 + tid;
+            at[0] = b;
             at[1] = (int)(t0 - (long long)before * pl.groups);
         }
-        done += t;
+    };
+    if (B <= NT) look(tid, n_mine, before_mine);
+    else {
+        int done = 0;
+        for (int b0 = 0; b0 < B; b0 += NT) {
+            int t;
+            const int n = tiles_of(b0 + tid), before = done + cta_scan(n, &t);
+            look(b0 + tid, n, before);
+            done += t;
+        }
     }
     __syncthreads();
     int b = at[0], in_seq = at[1];          // the share begins with tile in_seq (counted over the groups) of sequence b
@@ -189,35 +197,6 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
             const int u = grp * pl.wh + wu;
             if (u >= pl.units) continue;
             const int kh = u / pl.gt, h0 = u % pl.gt * 8, heads = min(8, G - h0);
-
-            // queries: lane (g8, t4) holds values 16 k + 2 t4 + {0, 1, 8, 9} of head h0 + g8
-            uint32_t qh[KS][2], ql[SPLIT ? KS : 1][2];
-            const QT* qrow = q + ((long long)b * n_q + kh * G + h0 + g8) * D + t4 * 2;
-            float top = 0.0f;
-            if (g8 < heads)
-                for (int i = 0; i < KS * 2; ++i) {
-                    float v[2];
-                    load_vals(qrow + i * 8, v);
-                    top = fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1])));
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = q_exponent(top);
-#pragma unroll
-            for (int i = 0; i < KS; ++i)
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    float v[2] = {0.0f, 0.0f};
-                    if (g8 < heads) load_vals(qrow + i * 16 + p * 8, v);
-                    v[0] = ldexpf(v[0], e);
-                    v[1] = ldexpf(v[1], e);
-                    uint32_t lo;
-                    split16(v[0], v[1], &qh[i][p], &lo);
-                    if constexpr (SPLIT) ql[i][p] = lo;
-                }
-            // score = S c in powers of two; this lane's columns of S^T are heads 2 t4 and 2 t4 + 1
-            const float c_own = ldexpf(scale2, -e);
-            const float c0 = __shfl_sync(0xffffffffu, c_own, t4 * 8), c1 = __shfl_sync(0xffffffffu, c_own, t4 * 8 + 4);
 
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f, o[KS][4];
 #pragma unroll
@@ -280,6 +259,35 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                 if (k0 + s < k1) seen[s] = fetch(s, k0 + s, at);
                 if (!BOX) cp_async_commit();
             }
+            // queries: lane (g8, t4) holds values 16 k + 2 t4 + {0, 1, 8, 9} of head h0 + g8
+            uint32_t qh[KS][2], ql[SPLIT ? KS : 1][2];
+            const QT* qrow = q + ((long long)b * n_q + kh * G + h0 + g8) * D + t4 * 2;
+            float top = 0.0f;
+            if (g8 < heads)
+                for (int i = 0; i < KS * 2; ++i) {
+                    float v[2];
+                    load_vals(qrow + i * 8, v);
+                    top = fmaxf(top, fmaxf(fabsf(v[0]), fabsf(v[1])));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = q_exponent(top);
+#pragma unroll
+            for (int i = 0; i < KS; ++i)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    float v[2] = {0.0f, 0.0f};
+                    if (g8 < heads) load_vals(qrow + i * 16 + p * 8, v);
+                    v[0] = ldexpf(v[0], e);
+                    v[1] = ldexpf(v[1], e);
+                    uint32_t lo;
+                    split16(v[0], v[1], &qh[i][p], &lo);
+                    if constexpr (SPLIT) ql[i][p] = lo;
+                }
+            // score = S c in powers of two; this lane's columns of S^T are heads 2 t4 and 2 t4 + 1
+            const float c_own = ldexpf(scale2, -e);
+            const float c0 = __shfl_sync(0xffffffffu, c_own, t4 * 8), c1 = __shfl_sync(0xffffffffu, c_own, t4 * 8 + 4);
+
             for (int k = k0; k < k1; k += ST) {
 #pragma unroll
                 for (int s = 0; s < ST; ++s) {       // stages by constant index

@@ -20,14 +20,17 @@ using PromptTiles = Tiles<D, D == 256 ? 1 : 2, D < 128 ? D : 128, D == 64 ? 8 : 
 template <int D>
 constexpr int PROMPT_OUT = D == 64 ? 8 * 2048 : 0;
 
-// What a CTA works on next: one or two query tiles of a sequence. Two are the same rows of two heads that share a key head
-// (pair: the group has an even number of heads; both tiles then see the same keys), or 256 rows of one head.
+// What a CTA works on next. Two query tiles are 256 rows of one head (BY_ROWS), or the same rows of two heads that share a key
+// head (BY_HEADS: the group has an even number of heads; both tiles then see the same keys). BY_KEYS there is one query tile,
+// even and odd key tiles take the places of the two, and both softmax halves join what they found: half the way for a tile
+// with many keys, for calls that have too few tiles to fill the device otherwise.
+enum { BY_ROWS = 0, BY_HEADS = 1, BY_KEYS = 2 };
 struct PromptItem {
     int h, first, q0, end;      // head; the sequence's first row; the first query row; the sequence's end
     int n[2];                   // key tiles per query tile; n[0] == 0: there is nothing more
 };
 struct PromptBars {
-    unsigned long long item_full[2], item_empty[2], q_empty[2], asked;
+    unsigned long long item_full[2], item_empty[2], q_empty[2], asked, ml_full, o_read;
     uint4 answer;               // of the work distributor, 16 bytes
     PromptItem item[2];
 };
@@ -56,15 +59,16 @@ __device__ __forceinline__ int block_answer(PromptBars& pb) {   // the block's i
 // the schedule warp has looked up the next block, its first K and V tiles are on their way, and the tensor cores begin as
 // soon as the last scores against the query tile are done. (One CTA per block: 61 sequences of 200 rows, 16 heads of 64, took 98 us, most of
 // it the way from a CTA's start to its first product and from its last to its end.)
-template <int D, typename T>
+template <int D, typename T, int MODE>
 __global__ void __launch_bounds__(PromptTiles<D, T>::WARPS * 32, 1)
 k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
               const T* q, const T* k, const T* v, T* out, const int* seq_start, int n_seqs, int rows, int n_q, int G,
-              long long q_stride, long long k_stride, long long v_stride, float scale2, int n_slots, int pair) {
+              long long q_stride, long long k_stride, long long v_stride, float scale2, int n_slots) {
     using Ti = PromptTiles<D, T>;
     constexpr int NQ = D == 256 ? 1 : 2, SC = D < 128 ? D : 128;
-    const int ROWS = NQ == 2 && !pair ? 2 * TILE_ROWS : TILE_ROWS, n_heads = pair ? n_q / 2 : n_q;   // rows and heads of a block
-    const int dh = pair ? 1 : 0, dq = pair ? 0 : TILE_ROWS;          // from the first query tile to the second
+    constexpr int ROWS = NQ == 2 && MODE == BY_ROWS ? 2 * TILE_ROWS : TILE_ROWS;                       // of a block
+    constexpr int dh = MODE == BY_HEADS ? 1 : 0, dq = MODE == BY_ROWS ? TILE_ROWS : 0;                // from one query tile to the other
+    const int n_heads = MODE == BY_HEADS ? n_q / 2 : n_q;
     extern __shared__ unsigned char smem_raw[];
     __shared__ TileBars bars;
     __shared__ PromptBars pb;
@@ -78,9 +82,11 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         for (int i = 0; i < 2; ++i) {
             mbar_init(&pb.item_full[i], 1);
             mbar_init(&pb.item_empty[i], NQ * 4 + 2);
-            mbar_init(&pb.q_empty[i], PROMPT_OUT<D> ? 1 : 4);
+            mbar_init(&pb.q_empty[i], PROMPT_OUT<D> ? 1 : MODE == BY_KEYS ? 8 : 4);
         }
         mbar_init(&pb.asked, 1);
+        mbar_init(&pb.ml_full, 8);
+        mbar_init(&pb.o_read, 8);
         mbar_fence_init();
     }
     Ti::setup(bars, 1);
@@ -136,7 +142,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                     it.q0 = first + tile * ROWS;
                     it.end = end;
 #pragma unroll
-                    for (int i = 0; i < NQ; ++i) {      // those up to the last row's own place
+                    for (int i = 0; i < (MODE == BY_KEYS ? 1 : NQ); ++i) {   // those up to the last row's own place
                         const int a = it.q0 + i * dq;
                         it.n[i] = a < end ? (min(a + TILE_ROWS, end) - 1 - first) / TILE_ROWS + 1 : 0;
                     }
@@ -182,9 +188,11 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 if (lane < D / CHUNK)
                     tma_3d(smem + i * Ti::QTILE + lane * CHUNK_BYTES, &mq, lane * CHUNK, it.h + i * dh, it.q0 + i * dq, &bars.q_full[i]);
             }
+            if (MODE == BY_KEYS && n_all > 1) put(&mk, 1);
             for (int j = 0; j < n_all; ++j) {
-                if (j + 1 < n_all) put(&mk, j + 1);
+                if (MODE != BY_KEYS && j + 1 < n_all) put(&mk, j + 1);
                 put(&mv, j);
+                if (MODE == BY_KEYS && j + 2 < n_all) put(&mk, j + 2);
             }
         }
     } else if (warp == NQ * 4) {
@@ -192,7 +200,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         TileFlow f;
         PromptItem it;
         while (next_item(&it))
-            if (!Ti::products(bars, smem, ring, it.n[0], it.n[1], f, PROMPT_OUT<D> ? pb.q_empty : nullptr)) break;
+            if (!Ti::template products<MODE == BY_KEYS>(bars, smem, ring, it.n[0], it.n[1], f, PROMPT_OUT<D> ? pb.q_empty : nullptr)) break;
     } else if (warp < NQ * 4) {
         Ti::many_registers();
         // ---- softmax: thread = row
@@ -200,46 +208,81 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         TileFlow f;
         PromptItem it;
         while (next_item(&it)) {
-            const int tiles = i ? it.n[1] : it.n[0], h = it.h + i * dh, first = it.first, end = it.end, t0 = it.q0 + i * dq, row = t0 + r;
+            const int h = it.h + i * dh, first = it.first, end = it.end, t0 = it.q0 + i * dq, row = t0 + r;
+            // this half's key tiles: j0, j0 + dj, ... below `tiles`
+            constexpr int dj = MODE == BY_KEYS ? 2 : 1;
+            const int tiles = MODE != BY_KEYS && i ? it.n[1] : it.n[0], j0 = MODE == BY_KEYS ? i : 0;
             if (tiles == 0) continue;
             float m = -INFINITY, l = 0.0f;
             bool ok = true;
-            for (int j = 0; j < tiles && ok; ++j) {
+            for (int j = j0; j < tiles && ok; j += dj) {
                 const int seen = row - first - j * TILE_ROWS;   // the last key of this tile that the row sees
-                ok = Ti::softmax_step(bars, i, j == 0, j + 1 == tiles, f, scale2, m, l, [&](uint32_t (&x)[128]) {
+                ok = Ti::softmax_step(bars, i, j == j0, j + dj >= tiles, f, scale2, m, l, [&](uint32_t (&x)[128]) {
                     if (j + 1 == tiles)   // (uniform) only a query tile's last key tile reaches past any of its rows
 #pragma unroll
                         for (int e = 0; e < 128; ++e)
                             if (e > seen) x[e] = 0xff800000u;
                 });
             }
-            if (!ok || !warp_wait(&bars.o_full[i], f.items[0] & 1, &bars.dead)) break;
+            if (!ok) break;
+            // the weights of the two halves' O, 1 / l included
+            float w0 = 1.0f, w1 = 0.0f;
+            if constexpr (MODE == BY_KEYS) {
+                float2* ml = reinterpret_cast<float2*>(smem + Ti::QTILE);   // (where a second query tile would be)
+                ml[i * TILE_ROWS + r] = make_float2(m, l);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pb.ml_full);
+                if (!warp_wait(&pb.ml_full, f.items[0] & 1, &bars.dead) || !warp_wait(&bars.o_full[0], f.items[0] & 1, &bars.dead)) break;
+                if (tiles > 1 && !warp_wait(&bars.o_full[1], f.items[1] & 1, &bars.dead)) break;
+                const float2 a = ml[r], b = ml[TILE_ROWS + r];
+                const float top = fmaxf(a.x, b.x);
+                w0 = a.x == -INFINITY ? 0.0f : ex2((a.x - top) * scale2);
+                w1 = b.x == -INFINITY ? 0.0f : ex2((b.x - top) * scale2);
+                const float inv = 1.0f / (w0 * a.y + w1 * b.y);
+                w0 *= inv;
+                w1 *= inv;
+                if (tiles > 1) ++f.items[1];
+            } else {
+                if (!warp_wait(&bars.o_full[i], f.items[0] & 1, &bars.dead)) break;
+                w0 = 1.0f / l;
+            }
             ++f.items[0];
             tc_fence_after();
-            // O / l through shared memory, CW columns at a time, so that the rows' stretches leave the warp together
+            // O / l through shared memory, CW columns at a time, so that the rows' stretches leave the warp together. BY_KEYS
+            // each half writes half of the columns.
             constexpr bool BUF = PROMPT_OUT<D> > 0;
-            constexpr int CW = BUF ? 32 : D, UNITS = CW / 8;
-            const uint32_t o_addr = bars.tmem + 256 + i * D + ((uint32_t)(threadIdx.x & 96) << 16);
-            unsigned char* mine = BUF ? ring + Ti::RING + warp * 2048 : smem + (i * TILE_ROWS + (warp & 3) * 32) * (D * 2);
-            const float inv = 1.0f / l;
+            constexpr int COLS = MODE == BY_KEYS ? D / 2 : D, CW = BUF ? 32 : COLS, UNITS = CW / 8, ROW = BUF ? CW * 2 : D * 2;
+            const int at0 = MODE == BY_KEYS ? i * COLS : 0;
+            const uint32_t o_addr = bars.tmem + 256 + (MODE == BY_KEYS ? 0 : i * D) + at0 + ((uint32_t)(threadIdx.x & 96) << 16);
+            unsigned char* mine = BUF ? ring + Ti::RING + warp * 2048
+                                      : smem + ((MODE == BY_KEYS ? 0 : i * TILE_ROWS) + (warp & 3) * 32) * (D * 2) + at0 * 2;
             bool bad = false;
-            for (int c0 = 0; c0 < D; c0 += CW) {
+            for (int c0 = 0; c0 < COLS; c0 += CW) {
                 for (int c = 0; c < CW; c += 32) {
-                    uint32_t o[32];
+                    uint32_t o[32], o1[MODE == BY_KEYS ? 32 : 1];
                     tmem_ld32(o_addr + c0 + c, o);
+                    if constexpr (MODE == BY_KEYS) {
+                        if (tiles > 1) tmem_ld32(o_addr + D + c0 + c, o1);
+                    }
                     tmem_ld_wait();
                     tmem_pin(o);
+                    if constexpr (MODE == BY_KEYS) {
+                        if (tiles > 1) tmem_pin(o1);
+                    }
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         float y[8];
 #pragma unroll
                         for (int t = 0; t < 8; ++t) {
-                            y[t] = __uint_as_float(o[e + t]) * inv;
+                            y[t] = __uint_as_float(o[e + t]) * w0;
+                            if constexpr (MODE == BY_KEYS) {
+                                if (tiles > 1) y[t] = fmaf(__uint_as_float(o1[e + t]), w1, y[t]);
+                            }
                             bad |= !(fabsf(y[t]) < INFINITY);
                         }
                         // (units of 16 bytes, stirred so that neither eight lanes' rows nor eight units share a bank)
                         const int u = (c + e) / 8, at = BUF ? u ^ (lane >> 1 & 3) : u ^ (lane & 7);
-                        *reinterpret_cast<uint4*>(mine + lane * (CW * 2) + at * 16) = Io<T>::pack(y);
+                        *reinterpret_cast<uint4*>(mine + lane * ROW + at * 16) = Io<T>::pack(y);
                     }
                 }
                 __syncwarp();
@@ -247,15 +290,20 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 for (int e = lane; e < 32 * UNITS; e += 32) {
                     const int rr = e / UNITS, u = e % UNITS, t = t0 + (warp & 3) * 32 + rr;
                     const int at = BUF ? u ^ (rr >> 1 & 3) : u ^ (rr & 7);
-                    const uint4 y = *reinterpret_cast<const uint4*>(mine + rr * (CW * 2) + at * 16);
-                    if (t < end) st_stream(reinterpret_cast<unsigned char*>(out + ((long long)t * n_q + h) * D + c0) + u * 16, y);
+                    const uint4 y = *reinterpret_cast<const uint4*>(mine + rr * ROW + at * 16);
+                    if (t < end) st_stream(reinterpret_cast<unsigned char*>(out + ((long long)t * n_q + h) * D + at0 + c0) + u * 16, y);
                 }
                 __syncwarp();
             }
             if (!BUF) {   // the query tile's memory may take the next one
                 fence_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&pb.q_empty[i]);
+                if (lane == 0) mbar_arrive(&pb.q_empty[MODE == BY_KEYS ? 0 : i]);
+            }
+            if constexpr (MODE == BY_KEYS) {   // neither half may write the next O (nor its m and l) before both have read these
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pb.o_read);
             }
             // A weight of 0 times a non-finite v is not 0 on the tensor cores: rows that came out non-finite are computed again
             // from the keys they may see alone
@@ -265,7 +313,11 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 const int t = t0 + (warp & 3) * 32 + __ffs(again) - 1;
                 again &= again - 1;
                 attn_row_prompt<D, T>(q + t * q_stride + h * D, k + first * k_stride + h / G * D, v + first * v_stride + h / G * D,
-                                      k_stride, v_stride, t - first + 1, scale2, out + ((long long)t * n_q + h) * D);
+                                      k_stride, v_stride, t - first + 1, scale2, out + ((long long)t * n_q + h) * D,
+                                      MODE != BY_KEYS ? 0xffffffffu : i ? 0xffff0000u : 0xffffu);
+            }
+            if constexpr (MODE == BY_KEYS) {
+                if (!warp_wait(&pb.o_read, (f.items[0] - 1) & 1, &bars.dead)) break;
             }
         }
     } else {

@@ -76,10 +76,10 @@ __device__ __forceinline__ float warp_dot(const float (&a)[N], const float (&b)[
     return s;
 }
 
-// Row of a prompt: query q, keys k0 + j k_stride, j < n
+// Row of a prompt: query q, keys k0 + j k_stride, j < n; `mine` says which lanes write
 template <int D, typename T>
 __device__ void attn_row_prompt(const T* q, const T* k0, const T* v0, long long k_stride, long long v_stride, int n, float scale2,
-                                T* out) {
+                                T* out, unsigned mine) {
     constexpr int N = D / 32;
     const int c = (threadIdx.x & 31) * N;
     float qv[N], kv[N], vv[N];
@@ -93,7 +93,7 @@ __device__ void attn_row_prompt(const T* q, const T* k0, const T* v0, long long 
     const float r = st.l > 0.0f ? 1.0f / st.l : (st.l == 0.0f ? 0.0f : st.l);
 #pragma unroll
     for (int i = 0; i < N; ++i) st.o[i] *= r;
-    store_vals(out + c, st.o);
+    if (mine >> (threadIdx.x & 31) & 1) store_vals(out + c, st.o);
 }
 
 }  // namespace b200

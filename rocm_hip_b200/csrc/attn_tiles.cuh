@@ -140,6 +140,9 @@ struct Tiles {
 
     // One warp: everything the tensor cores do for n0 / n1 key tiles of the query tiles. The ring brings
     // K 0, K 1, V 0, K 2, V 1, ...  q_empty: told when a query tile's last scores are done. False: given up.
+    // KEYS: there is one query tile, and its n0 key tiles go to the two S and O in turn, as two query tiles' would; the ring
+    // brings K 0, K 1, V 0, K 2, V 1, K 3, ...
+    template <bool KEYS = false>
     static __device__ __forceinline__ bool products(TileBars& bars, const unsigned char* qs, const unsigned char* ring, int n0, int n1,
                                                     TileFlow& f, unsigned long long* q_empty = nullptr) {
         constexpr uint32_t id_s = idesc_f16<T>(TILE_ROWS, false), id_o = idesc_f16<T>(SC, true);
@@ -164,7 +167,7 @@ struct Tiles {
 #pragma unroll
                 for (int p = 0; p < PARTS; ++p) mma_commit(&bars.empty[after(stage, p)]);
         };
-        const auto score = [&](int i, int buf, int stage) {   // S[buf] = Q_i K^T
+        const auto score = [&](int i, int buf, int stage) {   // S[buf] = Q_i K^T, Q_0 if KEYS
             const uint32_t d = tmem + buf * 128;
             if (elect_one()) {
 #pragma unroll
@@ -172,7 +175,7 @@ struct Tiles {
                     const uint32_t b = k_desc + after(stage, c / (SC / CHUNK)) * (STAGE >> 4) + c % (SC / CHUNK) * (CHUNK_BYTES >> 4);
 #pragma unroll
                     for (int z = 0; z < Z; ++z) {
-                        const uint32_t a = q_desc + (i * Z + z) * (QTILE >> 4) + c * (CHUNK_BYTES >> 4);
+                        const uint32_t a = q_desc + ((KEYS ? 0 : i) * Z + z) * (QTILE >> 4) + c * (CHUNK_BYTES >> 4);
 #pragma unroll
                         for (int e = 0; e < CHUNK / 16; ++e) mma_ss(d, a + e * 2, b + e * 2, id_s, c + e + z > 0);
                     }
@@ -195,6 +198,46 @@ struct Tiles {
             }
         };
         int ks = take(), vs;
+        if constexpr (KEYS) {
+            static_assert(NQ == 2, "two S and two O");
+            dead = dead || !warp_wait(&bars.q_full[0], f.items[0] & 1, &bars.dead);
+            if (dead) return false;
+            tc_fence_after();
+            score(0, 0, ks);
+            give(ks);
+            if (n0 > 1) {
+                ks = take();
+                if (dead) return false;
+                score(1, 1, ks);
+                give(ks);
+            }
+            if (q_empty && n0 <= 2 && elect_one()) mma_commit(&q_empty[0]);
+            for (int j = 0; j < n0; ++j) {
+                const int i = j & 1;
+                const unsigned par = (i ? f.steps[1] : f.steps[0]) & 1;
+                vs = take();
+                dead = dead || !warp_wait(&bars.p_half[i], par, &bars.dead);
+                if (dead) return false;
+                tc_fence_after();
+                join(i, i, vs, j > 1, 0, 4);
+                dead = dead || !warp_wait(&bars.p_full[i], par, &bars.dead);
+                if (dead) return false;
+                tc_fence_after();
+                join(i, i, vs, true, 4, 8);
+                if (i) ++f.steps[1]; else ++f.steps[0];
+                if (j + 2 >= n0 && elect_one()) mma_commit(&bars.o_full[i]);
+                give(vs);
+                if (j + 2 < n0) {
+                    ks = take();
+                    if (dead) return false;
+                    score(i, i, ks);
+                    if (q_empty && j + 3 == n0 && elect_one()) mma_commit(&q_empty[0]);
+                    give(ks);
+                }
+            }
+            ++f.items[0];
+            return true;
+        }
 #pragma unroll
         for (int i = 0; i < NQ; ++i) {
             if ((i ? n1 : n0) == 0) continue;

@@ -3,10 +3,10 @@
 // count is 0, and pages are always taken lowest id first, so the same calls give the same tables and a freed page needs
 // no list of its own.
 //
-// A call is a control kernel and a copy kernel. The control kernel is ONE cluster of KVP_CTAS CTAs: it has little to do
-// (a few words per sequence and page), what costs is the number of dependent passes over it, and a cluster's barrier
-// orders those passes without a launch in between. It leaves a list of (from, to) pages; the copy kernel, on the whole
-// device, moves them.
+// A call is a control kernel and a copy kernel. The control kernel is one CTA or ONE cluster of eight (CTAS): it has little to
+// do (a few words per sequence and page), what costs is the number of dependent passes over it, and a barrier of the CTA or
+// the cluster orders those passes without a launch in between. It leaves a list of (from, to) pages; the copy kernel, on
+// the whole device, moves them.
 
 #ifndef B200_KV_PAGES_CUH
 #define B200_KV_PAGES_CUH
@@ -16,10 +16,10 @@
 
 namespace b200 {
 
-constexpr int KVP_CTAS = 8, KVP_THREADS = 1024;
+constexpr int KVP_THREADS = 1024;
 constexpr int KVP_HEAD = 64;    // ints at the start of the work memory (below)
 
-// info[0] / the call's result, tested in this order
+// info[0]: what became of the call
 enum { KVP_OK = 0, KVP_FULL = 1, KVP_BAD = 2 };
 
 // Work memory: head [0 .. 15] free (or live) pages in each CTA's range, [16 .. 31] and [32 .. 47] holes and movers
@@ -34,36 +34,56 @@ struct KvPagesWork {
     static size_t ints(int n_seqs, int n_pages) { return KVP_HEAD + 3 * (size_t)n_seqs + 3 * (size_t)n_pages; }
 };
 
-__device__ __forceinline__ void kvp_sync() {   // all threads of the cluster; orders their global accesses too
-    __threadfence();
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+// All threads of the CTA or cluster; orders their global accesses too
+template <int CTAS>
+__device__ __forceinline__ void kvp_sync() {
+    if constexpr (CTAS == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
-// Exclusive sum over the CTA in thread order, and the total. Two barriers; part: 33 ints.
-__device__ __forceinline__ int kvp_scan(int v, int* total, int* part) {
+// Exclusive sums over the CTA in thread order of N values at once, and their totals. Two barriers; part: N * 32 ints.
+template <int N>
+__device__ __forceinline__ void kvp_scan(int (&v)[N], int (&total)[N], int* part) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    int x = v;
+    int own[N];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
+    for (int k = 0; k < N; ++k) own[k] = v[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const int y = __shfl_up_sync(0xffffffffu, v[k], o);
+            if (lane >= o) v[k] += y;
+        }
     __syncthreads();
-    if (lane == 31) part[w] = x;
+    if (lane == 31)
+#pragma unroll
+        for (int k = 0; k < N; ++k) part[k * 32 + w] = v[k];
     __syncthreads();
-    int base = 0, all = 0;
-    for (int i = 0; i < KVP_THREADS / 32; ++i) {
-        const int p = part[i];
-        base += i < w ? p : 0;
-        all += p;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {      // every warp sums the warps' totals
+        const int mine = part[k * 32 + lane];
+        int x = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        total[k] = __shfl_sync(0xffffffffu, x, 31);
+        v[k] += __shfl_sync(0xffffffffu, x - mine, w) - own[k];
     }
-    *total = all;
-    return base + x - v;
+}
+__device__ __forceinline__ int kvp_scan1(int v, int* total, int* part) {
+    int a[1] = {v}, t[1];
+    kvp_scan<1>(a, t, part);
+    *total = t[0];
+    return a[0];
 }
 
 // The CTA's share of the pages: [*a, *b)
+template <int CTAS>
 __device__ __forceinline__ void kvp_range(int n_pages, int cta, int* a, int* b) {
-    const int per = ((n_pages + KVP_CTAS - 1) / KVP_CTAS + 3) / 4 * 4;
+    const int per = (n_pages + CTAS - 1) / CTAS;
     *a = min(n_pages, cta * per);
     *b = min(n_pages, *a + per);
 }
@@ -73,7 +93,7 @@ template <typename F>
 __device__ __forceinline__ int kvp_count(const int* refs, int a, int b, int* part, F test) {
     int n = 0, total;
     for (int p = a + threadIdx.x; p < b; p += KVP_THREADS) n += test(p, refs[p]) ? 1 : 0;
-    kvp_scan(n, &total, part);
+    kvp_scan1(n, &total, part);
     return total;
 }
 
@@ -84,15 +104,16 @@ __device__ __forceinline__ void kvp_list(const int* refs, int a, int b, int base
         const int p = p0 + threadIdx.x;
         const bool yes = p < b && test(p, refs[p]);
         int total;
-        const int r = kvp_scan(yes ? 1 : 0, &total, part);
+        const int r = kvp_scan1(yes ? 1 : 0, &total, part);
         if (yes && base + r < limit) list[base + r] = p;
         base += total;
     }
 }
 
+template <int CTAS>
 __device__ __forceinline__ int kvp_before(const int* counts, int cta, int* all) {
     int base = 0, sum = 0;
-    for (int i = 0; i < KVP_CTAS; ++i) {
+    for (int i = 0; i < CTAS; ++i) {
         base += i < cta ? counts[i] : 0;
         sum += counts[i];
     }
@@ -120,14 +141,15 @@ __device__ __forceinline__ int kvp_pages(int n, int shift) { return (int)(((long
 
 // parent[s] >= 0: the empty sequence s becomes a copy of parent[s]. Whole pages are shared, a last page that is only
 // partly filled gets a copy of its own, so that both may grow.
+template <int CTAS>
 __global__ void __launch_bounds__(KVP_THREADS)
 k_kv_pages_fork(b200_kv_pages kv, const int* parent) {
-    __shared__ int part[33];
+    __shared__ int part[96];
     pdl_entry();
     const int cta = blockIdx.x, mask = (1 << kv.page_shift) - 1;
     const KvPagesWork w(kv.work, kv.n_seqs, kv.n_pages);
     int a, b;
-    kvp_range(kv.n_pages, cta, &a, &b);
+    kvp_range<CTAS>(kv.n_pages, cta, &a, &b);
     const auto is_free = [](int, int r) { return r == 0; };
     const int mine = kvp_count(kv.refs, a, b, part, is_free);
     if (threadIdx.x == 0) w.head[cta] = mine;
@@ -149,23 +171,23 @@ k_kv_pages_fork(b200_kv_pages kv, const int* parent) {
                 w.soff[s] = n;   // the parent's length, or -1
             }
             int total;
-            const int r = kvp_scan(need, &total, part);
+            const int r = kvp_scan1(need, &total, part);
             if (s < kv.n_seqs) w.off[s] = base + r;
             base += total;
         }
         bad = __syncthreads_or(bad);
         if (threadIdx.x == 0) { w.head[48] = base; w.head[49] = bad; }
     }
-    kvp_sync();
+    kvp_sync<CTAS>();
     int n_free;
-    const int before = kvp_before(w.head, cta, &n_free), need = w.head[48];
+    const int before = kvp_before<CTAS>(w.head, cta, &n_free), need = w.head[48];
     const int status = w.head[49] ? KVP_BAD : need > n_free ? KVP_FULL : KVP_OK;
     if (status == KVP_OK) kvp_list(kv.refs, a, b, before, need, w.to, part, is_free);
-    kvp_sync();
+    kvp_sync<CTAS>();
     if (cta == 0 && threadIdx.x == 0) kvp_tell(kv, w.head, status, n_free - (status == KVP_OK ? need : 0), status == KVP_OK ? need : 0);
     if (status != KVP_OK) return;
     const int lane = threadIdx.x & 31;
-    for (int s = cta + KVP_CTAS * (threadIdx.x >> 5); s < kv.n_seqs; s += KVP_CTAS * (KVP_THREADS / 32)) {
+    for (int s = cta + CTAS * (threadIdx.x >> 5); s < kv.n_seqs; s += CTAS * (KVP_THREADS / 32)) {
         const int n = w.soff[s];
         if (n < 0) continue;
         const int* from = kv.table + (long long)parent[s] * kv.max_pages;
@@ -192,14 +214,15 @@ k_kv_pages_fork(b200_kv_pages kv, const int* parent) {
 // no longer needs; then the others take the pages they lack, in the order of the sequences, and the cache rows of
 // their new tokens go to slots. A last page that is partly filled and shared is replaced by a copy before it grows.
 // Where the pages do not suffice, or a length exceeds the table, no sequence grows.
+template <int CTAS>
 __global__ void __launch_bounds__(KVP_THREADS)
 k_kv_pages_resize(b200_kv_pages kv, const int* new_lens, int* slots, int n_slots) {
-    __shared__ int part[33];
+    __shared__ int part[96];
     pdl_entry();
     const int cta = blockIdx.x, mask = (1 << kv.page_shift) - 1, lane = threadIdx.x & 31;
     const long long cap = (long long)kv.max_pages << kv.page_shift;
     const KvPagesWork w(kv.work, kv.n_seqs, kv.n_pages);
-    const int s_first = cta + KVP_CTAS * (threadIdx.x >> 5), s_step = KVP_CTAS * (KVP_THREADS / 32);
+    const int s_first = cta + CTAS * (threadIdx.x >> 5), s_step = CTAS * (KVP_THREADS / 32);
     for (int s = s_first; s < kv.n_seqs; s += s_step) {
         const int to = new_lens[s], n = kvp_len(kv, s);
         if (to < 0 || to >= n) continue;
@@ -212,9 +235,9 @@ k_kv_pages_resize(b200_kv_pages kv, const int* new_lens, int* slots, int n_slots
         }
         if (lane == 0) kv.lens[s] = to;
     }
-    kvp_sync();
+    kvp_sync<CTAS>();
     int a, b;
-    kvp_range(kv.n_pages, cta, &a, &b);
+    kvp_range<CTAS>(kv.n_pages, cta, &a, &b);
     const auto is_free = [](int, int r) { return r == 0; };
     const int mine = kvp_count(kv.refs, a, b, part, is_free);
     if (threadIdx.x == 0) w.head[cta] = mine;
@@ -236,27 +259,26 @@ k_kv_pages_resize(b200_kv_pages kv, const int* new_lens, int* slots, int n_slots
                     }
                 }
             }
-            int total, stotal, ctotal;
-            const int r = kvp_scan(need + cow, &total, part), sr = kvp_scan(more, &stotal, part);
-            const int cr = kvp_scan(cow, &ctotal, part);
+            int rank[3] = {need + cow, more, cow}, total[3];
+            kvp_scan<3>(rank, total, part);
             if (s < kv.n_seqs) {
-                w.off[s] = base + r;
-                w.soff[s] = sbase + sr;
-                w.coff[s] = cow ? cbase + cr : -1;
+                w.off[s] = base + rank[0];
+                w.soff[s] = sbase + rank[1];
+                w.coff[s] = cow ? cbase + rank[2] : -1;
             }
-            base += total;
-            sbase += stotal;
-            cbase += ctotal;
+            base += total[0];
+            sbase += total[1];
+            cbase += total[2];
         }
         bad = __syncthreads_or(bad);
         if (threadIdx.x == 0) { w.head[48] = base; w.head[49] = bad; w.head[50] = sbase; w.head[51] = cbase; }
     }
-    kvp_sync();
+    kvp_sync<CTAS>();
     int n_free;
-    const int before = kvp_before(w.head, cta, &n_free), need = w.head[48], n_new = w.head[50], copies = w.head[51];
+    const int before = kvp_before<CTAS>(w.head, cta, &n_free), need = w.head[48], n_new = w.head[50], copies = w.head[51];
     const int status = w.head[49] ? KVP_BAD : need > n_free ? KVP_FULL : KVP_OK;
     if (status == KVP_OK) kvp_list(kv.refs, a, b, before, need, w.list, part, is_free);
-    kvp_sync();
+    kvp_sync<CTAS>();
     if (status != KVP_OK) {
         if (cta == 0 && threadIdx.x == 0) kvp_tell(kv, w.head, status, n_free, 0);
         return;
@@ -285,10 +307,10 @@ k_kv_pages_resize(b200_kv_pages kv, const int* new_lens, int* slots, int n_slots
         }
         if (lane == 0) kv.lens[s] = to;
     }
-    kvp_sync();
+    kvp_sync<CTAS>();
     if (slots) {   // a thread per new token: its sequence is the last whose first new token is not behind it
         const int n_out = min(n_new, n_slots);
-        for (int i = cta * KVP_THREADS + threadIdx.x; i < n_out; i += KVP_CTAS * KVP_THREADS) {
+        for (int i = cta * KVP_THREADS + threadIdx.x; i < n_out; i += CTAS * KVP_THREADS) {
             int lo = 0, hi = kv.n_seqs;
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
@@ -299,48 +321,53 @@ k_kv_pages_resize(b200_kv_pages kv, const int* new_lens, int* slots, int n_slots
             slots[i] = (kv.table[(long long)s * kv.max_pages + (t >> kv.page_shift)] << kv.page_shift) + (t & mask);
         }
     }
+    if (copies == 0) {
+        if (cta == 0 && threadIdx.x == 0) kvp_tell(kv, w.head, KVP_OK, n_free - need, 0);
+        return;
+    }
     // pages whose last reader took a copy are free again: none of them was handed out by this call
     const int left = kvp_count(kv.refs, a, b, part, is_free);
     if (threadIdx.x == 0) w.head[16 + cta] = left;
-    kvp_sync();
+    kvp_sync<CTAS>();
     if (cta == 0 && threadIdx.x == 0) {
         int all;
-        kvp_before(w.head + 16, 0, &all);
+        kvp_before<CTAS>(w.head + 16, 0, &all);
         kvp_tell(kv, w.head, KVP_OK, all, copies);
     }
 }
 
 // The n_live pages in use become pages 0 .. n_live - 1: those at or behind n_live move, in ascending order, into the
 // free ids before it. No page is both moved from and moved to.
+template <int CTAS>
 __global__ void __launch_bounds__(KVP_THREADS)
 k_kv_pages_compact(b200_kv_pages kv) {
-    __shared__ int part[33];
+    __shared__ int part[96];
     pdl_entry();
     const int cta = blockIdx.x, lane = threadIdx.x & 31;
     const KvPagesWork w(kv.work, kv.n_seqs, kv.n_pages);
     int a, b, n_live, n_holes, n_move;
-    kvp_range(kv.n_pages, cta, &a, &b);
+    kvp_range<CTAS>(kv.n_pages, cta, &a, &b);
     const int mine = kvp_count(kv.refs, a, b, part, [](int, int r) { return r > 0; });
     if (threadIdx.x == 0) w.head[cta] = mine;
-    kvp_sync();
-    kvp_before(w.head, cta, &n_live);
+    kvp_sync<CTAS>();
+    kvp_before<CTAS>(w.head, cta, &n_live);
     const auto hole = [n_live](int p, int r) { return r <= 0 && p < n_live; };
     const auto mover = [n_live](int p, int r) { return r > 0 && p >= n_live; };
     const int h = kvp_count(kv.refs, a, b, part, hole), m = kvp_count(kv.refs, a, b, part, mover);
     if (threadIdx.x == 0) { w.head[16 + cta] = h; w.head[32 + cta] = m; }
-    kvp_sync();
-    const int hb = kvp_before(w.head + 16, cta, &n_holes), mb = kvp_before(w.head + 32, cta, &n_move);
+    kvp_sync<CTAS>();
+    const int hb = kvp_before<CTAS>(w.head + 16, cta, &n_holes), mb = kvp_before<CTAS>(w.head + 32, cta, &n_move);
     kvp_list(kv.refs, a, b, hb, kv.n_pages, w.to, part, hole);
     kvp_list(kv.refs, a, b, mb, kv.n_pages, w.from, part, mover);
     for (int p = max(a, n_live) + threadIdx.x; p < b; p += KVP_THREADS) w.list[p] = p;
-    kvp_sync();
-    for (int r = cta * KVP_THREADS + threadIdx.x; r < n_move; r += KVP_CTAS * KVP_THREADS) {
+    kvp_sync<CTAS>();
+    for (int r = cta * KVP_THREADS + threadIdx.x; r < n_move; r += CTAS * KVP_THREADS) {
         w.list[w.from[r]] = w.to[r];
         kv.refs[w.to[r]] = kv.refs[w.from[r]];
         kv.refs[w.from[r]] = 0;
     }
-    kvp_sync();
-    for (int s = cta + KVP_CTAS * (threadIdx.x >> 5); s < kv.n_seqs; s += KVP_CTAS * (KVP_THREADS / 32)) {
+    kvp_sync<CTAS>();
+    for (int s = cta + CTAS * (threadIdx.x >> 5); s < kv.n_seqs; s += CTAS * (KVP_THREADS / 32)) {
         int* row = kv.table + (long long)s * kv.max_pages;
         const int used = kvp_pages(kvp_len(kv, s), kv.page_shift);
         for (int i = lane; i < used; i += 32) {

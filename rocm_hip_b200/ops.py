@@ -53,6 +53,15 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _stream_of(t):
+    """The current stream as an int, for the calls whose latency counts (a Stream object costs as much as a launch). The
+    launchers run on the current device: a tensor of another one is refused."""
+    dev = torch.cuda.current_device()
+    if t.get_device() != dev:
+        raise ValueError(f"tensor on device {t.get_device()}, current device {dev}")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def gpu_ops_init(co_path="gpu_ops.co"):
     return _lib.load().gpu_ops_init(co_path.encode())
 
@@ -400,7 +409,7 @@ def gpu_attn_prompt(q, k, v, out, seq_start, n_seqs, T, n_q, n_kv, head_dim, sca
     lib = _lib.load()
     fn = lib.gpu_attn_prompt_bf16 if q.dtype == torch.bfloat16 else lib.gpu_attn_prompt_f16
     _check("gpu_attn_prompt", fn(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(seq_start), n_seqs, T, n_q, n_kv, head_dim, q_stride,
-                                 k_stride, v_stride, scale, _stream()))
+                                 k_stride, v_stride, scale, _stream_of(q)))
 
 
 def gpu_attn_decode_scratch_bytes(n_q, n_kv, head_dim, B, prefix_len=0):
@@ -421,7 +430,7 @@ def gpu_attn_decode(q, K, V, kv_stride, kv_shift, kv_bstride, n_pages, pages, ma
     fn = lib.gpu_attn_decode if q.dtype == torch.float32 else lib.gpu_attn_decode_bf16
     _check("gpu_attn_decode", fn(_ptr(q), _ptr(K), _ptr(V), kv_stride, kv_shift, kv_bstride, n_pages, _ptr(pages), max_pages, _ptr(lens),
                                  prefix_len, _ptr(out), n_q, n_kv, head_dim, B, scale, _ptr(scratch),
-                                 scratch.numel() * scratch.element_size(), _stream()))
+                                 scratch.numel() * scratch.element_size(), _stream_of(q)))
 
 
 class KvPages:
@@ -447,19 +456,19 @@ class KvPages:
 
 def gpu_kv_pages_fork(kv, parent):
     """parent int32 [n_seqs]: -1, or the sequence that the empty sequence s becomes a copy of."""
-    _check("gpu_kv_pages_fork", _lib.load().gpu_kv_pages_fork(C.byref(kv.struct()), _ptr(parent), _stream()))
+    _check("gpu_kv_pages_fork", _lib.load().gpu_kv_pages_fork(C.byref(kv.struct()), _ptr(parent), _stream_of(kv.table)))
 
 
 def gpu_kv_pages_resize(kv, new_lens, slots=None):
     """new_lens int32 [n_seqs]: the length each sequence gets (0 frees it, negative keeps it); slots (int32): receives the
     cache rows of the new tokens."""
     _check("gpu_kv_pages_resize", _lib.load().gpu_kv_pages_resize(C.byref(kv.struct()), _ptr(new_lens), _ptr(slots),
-                                                                  0 if slots is None else slots.numel(), _stream()))
+                                                                  0 if slots is None else slots.numel(), _stream_of(kv.table)))
 
 
 def gpu_kv_pages_compact(kv):
     """Moves the pages in use to the lowest ids."""
-    _check("gpu_kv_pages_compact", _lib.load().gpu_kv_pages_compact(C.byref(kv.struct()), _stream()))
+    _check("gpu_kv_pages_compact", _lib.load().gpu_kv_pages_compact(C.byref(kv.struct()), _stream_of(kv.table)))
 
 
 class HostRows:
