@@ -152,7 +152,7 @@ struct DecodePlan {
     long long px_rows;
     size_t first, own_ml, own_o, px_ml, px_o, bytes;
 
-    DecodePlan(int n_q, int n_kv, int D, int B, int prefix) {
+    DecodePlan(int n_q, int n_kv, int D, int B, int prefix, bool f32) {
         const int warps = D == 256 ? OwnShape<256>::WARPS : OwnShape<128>::WARPS, sms = sm_count();
         const OwnPlan own(n_q, n_kv, warps);
         grid_own = sms;
@@ -167,10 +167,14 @@ struct DecodePlan {
             row_tiles = (int)((M + nq * TILE_ROWS - 1) / (nq * TILE_ROWS));
             px_rows = (long long)row_tiles * nq * TILE_ROWS;
             // stretches of the prefix: as many as make the CTAs whole waves of the device, counting about four tiles' time
-            // for what a CTA does once (its queries, its result and the pieces' way through scratch)
+            // for what a CTA does once (its queries, its result and the pieces' way through scratch). For fp32 rows no
+            // longer than six tiles: the tensor cores cut sums off where fp32 arithmetic rounds, a stretch of t tiles
+            // (16 t additions) loses 2.5e-8 per addition, and joining stretches does not (8,192 rows, heads of 256: 3.5e-6
+            // with stretches of nine tiles, 2.6e-6 with six; 32,768 rows, heads of 128: 1.1e-5 with 37, 2.5e-6 with six).
             const int tiles = (prefix + TILE_ROWS - 1) / TILE_ROWS, base = n_kv * row_tiles;
+            const int least = f32 ? (tiles + 5) / 6 : 1;
             long long best = LLONG_MAX;
-            for (int s = 1; s <= tiles && s <= 64; ++s) {
+            for (int s = least; s <= tiles && s < least + 64; ++s) {
                 const long long cost = (((long long)base * s + sms - 1) / sms) * ((tiles + s - 1) / s + 4);
                 if (cost < best) { best = cost; splits = s; }
             }
@@ -247,7 +251,7 @@ cudaError_t launch_decode(const T* q, const uint16_t* K, const uint16_t* V, int 
         !al16(out) || (const void*)out == (const void*)q)
         return cudaErrorInvalidValue;
     if (prefix_len < 0 || prefix_len % (1 << kv_shift) || prefix_len > ((long long)max_pages << kv_shift)) return cudaErrorInvalidValue;
-    const DecodePlan pl(n_q, n_kv, D, B, prefix_len);
+    const DecodePlan pl(n_q, n_kv, D, B, prefix_len, sizeof(T) == 4);
     if (scratch_bytes < pl.bytes || !scratch || !al16(scratch)) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
     const PagedKv kv{reinterpret_cast<const __half*>(K), reinterpret_cast<const __half*>(V), pages, lens, kv_bstride, kv_stride,
@@ -326,7 +330,8 @@ int b200_attn_gave_up(void) {
 
 size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len) {
     if (!good_heads(n_q, n_kv, head_dim) || B < 1 || (long long)B * n_q > (1 << 28) || prefix_len < 0) return 0;
-    return DecodePlan(n_q, n_kv, head_dim, B, prefix_len).bytes;
+    const size_t a = DecodePlan(n_q, n_kv, head_dim, B, prefix_len, true).bytes, b = DecodePlan(n_q, n_kv, head_dim, B, prefix_len, false).bytes;
+    return a > b ? a : b;      // (serves both row types)
 }
 
 cudaError_t gpu_attn_decode(const float* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,

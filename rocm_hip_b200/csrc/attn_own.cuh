@@ -278,14 +278,14 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                 for (int p = 0; p < 2; ++p) {
                     float v[2] = {0.0f, 0.0f};
                     if (g8 < heads) load_vals(qrow + i * 16 + p * 8, v);
-                    v[0] = ldexpf(v[0], e);
-                    v[1] = ldexpf(v[1], e);
+                    v[0] = scale2e(v[0], e);
+                    v[1] = scale2e(v[1], e);
                     uint32_t lo;
                     split16(v[0], v[1], &qh[i][p], &lo);
                     if constexpr (SPLIT) ql[i][p] = lo;
                 }
             // score = S c in powers of two; this lane's columns of S^T are heads 2 t4 and 2 t4 + 1
-            const float c_own = ldexpf(scale2, -e);
+            const float c_own = scale2e(scale2, -e);
             const float c0 = __shfl_sync(0xffffffffu, c_own, t4 * 8), c1 = __shfl_sync(0xffffffffu, c_own, t4 * 8 + 4);
 
             for (int k = k0; k < k1; k += ST) {
@@ -367,8 +367,17 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                         for (int i = 0; i < KS; ++i) {
                             uint32_t a[4];
                             ldsm4t(smem_u32(Vt) + own_at((lane & 7) + (lane >> 4) * 8, i * 2 + (lane >> 3 & 1)), a);
-                            mma16(o[i], a, b0, b1);
-                            if constexpr (SPLIT) mma16(o[i], a, d0, d1);
+                            if constexpr (SPLIT) {
+                                // (the tensor cores cut a sum off where fp32 arithmetic rounds: over thousands of rows the sums
+                                // shrink, 2.0e-6 after 4,000 against 5.9e-7. So only a tile's own products are summed there.)
+                                float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma16(y, a, d0, d1);
+                                mma16(y, a, b0, b1);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[i][e] += y[e];
+                            } else {
+                                mma16(o[i], a, b0, b1);
+                            }
                         }
                         __syncwarp();
                     }

@@ -120,14 +120,14 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
                 const int x = q_exponent(top[t]);
-                if (lane == r8 + t) c_row = ldexpf(scale2, -x);
+                if (lane == r8 + t) c_row = scale2e(scale2, -x);
                 const int col = lane * N, in_tile = (warp & 3) * 32 + r8 + t;
                 unsigned char* at = smem + i * Ti::QTILE * (SPLIT ? 2 : 1) + col / CHUNK * CHUNK_BYTES + in_tile * 128 +
                                     (((col % CHUNK / 8) ^ (in_tile & 7)) * 16) + col % 8 * 2;
 #pragma unroll
                 for (int e = 0; e < N; e += 2) {
                     uint32_t hi, lo;
-                    split16(ldexpf(v[t][e], x), ldexpf(v[t][e + 1], x), &hi, &lo);
+                    split16(scale2e(v[t][e], x), scale2e(v[t][e + 1], x), &hi, &lo);
                     *reinterpret_cast<uint32_t*>(at + e * 2) = hi;
                     if constexpr (SPLIT) *reinterpret_cast<uint32_t*>(at + Ti::QTILE + e * 2) = lo;
                 }

@@ -158,6 +158,9 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     else return pack_f16(lo, hi);
 }
 
+// v 2^e for |e| < 250, exact but where the result is subnormal (two multiplications; ldexpf is twenty instructions)
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+__device__ __forceinline__ float scale2e(float v, int e) { return v * pow2(e / 2) * pow2(e - e / 2); }
 // v as fp16 hi (+ lo)
 __device__ __forceinline__ void split16(float a, float b, uint32_t* hi, uint32_t* lo) {
     const __half2 h = __floats2half2_rn(a, b);
