@@ -517,7 +517,8 @@ void b200_gguf_free_tensor(void* dev_ptr);
  * q [T][n_q * head_dim] as gpu_qk_norm_rope leaves it, k and v [T][n_kv * head_dim], bf16 or fp16 bit patterns; rows may
  * sit q_stride / k_stride / v_stride values apart (multiples of 8; 0: contiguous), e.g. in a fused q | k | v
  * projection. out [T][n_q * head_dim] is contiguous and shares no memory with the inputs. Empty sequences are
- * allowed; rows before the first and behind the last sequence are neither read into a result nor written. Weights are
+ * allowed; rows before the first and behind the last sequence are neither read into a result nor written, and a row's
+ * result depends on no k or v that it does not see, non-finite ones included. Weights are
  * rounded to the rows' type before they meet v (the sum of weights is not), out once. T <= 2^30; pointers 16-byte
  * aligned. */
 cudaError_t gpu_attn_prompt_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int* seq_start,
@@ -539,7 +540,9 @@ int b200_attn_gave_up(void);
  * [0, n_pages) are rows that are not seen. lens[b] <= 0: out[b] is zero.
  * prefix_len > 0: every sequence with lens[b] >= prefix_len begins with the same prefix_len rows IN THE SAME PAGES (as
  * gpu_kv_pages_fork leaves them), which are then read once for the whole batch; a multiple of 2^kv_shift. Sequences with
- * fewer rows (idle slots) use their own pages only. Memory behind lens[b] may hold anything.
+ * fewer rows (idle slots) use their own pages only. Memory behind lens[b] may hold anything; a page of up to 4096 rows is
+ * readable to its end, of larger ones (a contiguous cache: kv_shift 30, one page per sequence) nothing behind lens[b] is
+ * touched.
  * fp32 rows keep fp32 accuracy; kv_stride and kv_bstride are multiples of 8, pointers 16-byte aligned, out is not q.
  * scratch: device memory of gpu_attn_decode_scratch_bytes(...) bytes, any contents, in use until the call has run; calls
  * that may overlap need scratch of their own. */
@@ -564,7 +567,7 @@ typedef struct b200_kv_pages {
     int* refs;           /* [n_pages] sequences that hold the page */
     int* info;           /* [4] */
     int* work;           /* gpu_kv_pages_work_ints(n_seqs, n_pages) ints, any contents */
-    int n_seqs, max_pages, n_pages;
+    int n_seqs, max_pages, n_pages;   /* n_seqs * max_pages fits an int */
     int page_shift;      /* a page holds 2^page_shift rows; n_pages << page_shift fits an int */
     void* pool;          /* 16-byte aligned; page_bytes and part_stride multiples of 16 */
     size_t page_bytes;

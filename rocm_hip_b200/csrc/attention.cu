@@ -201,10 +201,12 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
     const OwnScratch sc{reinterpret_cast<int*>(scratch), reinterpret_cast<int*>(scratch + pl.first),
                         reinterpret_cast<float*>(scratch + pl.own_ml), reinterpret_cast<float*>(scratch + pl.own_o)};
     // The copy engine takes the cache apart where pages are whole swizzle atoms (8 rows) and a tensor map can describe it;
-    // else a prefix is read like every sequence's own rows, and those by the threads
+    // else a prefix is read like every sequence's own rows, and those by the threads. It fetches 16 rows at a time, so a
+    // sequence's last fetch may reach behind its rows, to the page's end at most: pages of more than 4,096 rows (a contiguous
+    // cache is one of 2^30) need not be memory up to there.
     CUtensorMap mk, mv, ok, ov;
-    const bool box = kv.kv_shift >= 3 && page_map(&ok, kv.K, D, n_kv, kv, 16) && page_map(&ov, kv.V, D, n_kv, kv, 16);
-    const bool shared = pl.splits > 0 && box && page_map(&mk, kv.K, D, n_kv, kv, TILE_ROWS) && page_map(&mv, kv.V, D, n_kv, kv, TILE_ROWS);
+    const bool box = kv.kv_shift >= 3 && kv.kv_shift <= 12 && page_map(&ok, kv.K, D, n_kv, kv, 16) && page_map(&ov, kv.V, D, n_kv, kv, 16);
+    const bool shared = pl.splits > 0 && kv.kv_shift >= 3 && page_map(&mk, kv.K, D, n_kv, kv, TILE_ROWS) && page_map(&mv, kv.V, D, n_kv, kv, TILE_ROWS);
     const PrefixScratch px{shared ? pl.splits : 0, pl.px_rows, reinterpret_cast<float*>(scratch + pl.px_ml),
                            reinterpret_cast<float*>(scratch + pl.px_o)};
     const int behind = shared ? prefix : 0;
@@ -272,7 +274,7 @@ bool good_pages(const b200_kv_pages* kv) {
            kv->n_pages > 0 && kv->page_shift >= 0 && kv->page_shift <= 30 &&
            ((long long)kv->n_pages << kv->page_shift) <= INT_MAX && kv->page_bytes > 0 && kv->page_bytes % 16 == 0 &&
            kv->page_bytes <= INT_MAX && kv->n_parts > 0 && (kv->n_parts == 1 || kv->part_stride >= kv->page_bytes * kv->n_pages) &&
-           kv->part_stride % 16 == 0 && al16(kv->pool) && (long long)kv->n_seqs * kv->max_pages <= (1LL << 40);
+           kv->part_stride % 16 == 0 && al16(kv->pool) && (long long)kv->n_seqs * kv->max_pages <= INT_MAX;
 }
 
 // How many CTAs the control kernel takes: one where its tables are small, so that the passes over them are separated by a

@@ -305,16 +305,28 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&pb.o_read);
             }
-            // A weight of 0 times a non-finite v is not 0 on the tensor cores: rows that came out non-finite are computed again
-            // from the keys they may see alone
+            // A weight of 0 times a non-finite v is not 0 on the tensor cores. Rows that came out non-finite are computed again from
+            // the keys they see, where a key of the last tile that they do not see has such a v.
             unsigned again = __ballot_sync(0xffffffffu, bad && row < end);
             __syncwarp();
-            while (again) {
-                const int t = t0 + (warp & 3) * 32 + __ffs(again) - 1;
-                again &= again - 1;
-                attn_row_prompt<D, T>(q + t * q_stride + h * D, k + first * k_stride + h / G * D, v + first * v_stride + h / G * D,
-                                      k_stride, v_stride, t - first + 1, scale2, out + ((long long)t * n_q + h) * D,
-                                      MODE != BY_KEYS ? 0xffffffffu : i ? 0xffff0000u : 0xffffu);
+            if (again) {
+                const int d0 = first + (tiles - 1) * TILE_ROWS;      // the last tile's first key
+                unsigned non_finite[4];
+                find_non_finite<D>(v + d0 * v_stride + h / G * D, v_stride, min(TILE_ROWS, rows - d0), non_finite);
+                while (again) {
+                    const int t = t0 + (warp & 3) * 32 + __ffs(again) - 1, seen = t - d0;
+                    again &= again - 1;
+                    bool unseen = false;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const int k = seen + 1 - 32 * w;             // first bit of this word that the row does not see
+                        unseen |= (k <= 0 ? non_finite[w] : k < 32 ? non_finite[w] >> k : 0) != 0;
+                    }
+                    if (unseen)
+                        attn_row_again<D, T>(q + t * q_stride + h * D, k + first * k_stride + h / G * D, v + first * v_stride + h / G * D,
+                                             k_stride, v_stride, t - first + 1, scale2, out + ((long long)t * n_q + h) * D,
+                                             MODE != BY_KEYS ? 0xffffffffu : i ? 0xffff0000u : 0xffffu);
+                }
             }
             if constexpr (MODE == BY_KEYS) {
                 if (!warp_wait(&pb.o_read, (f.items[0] - 1) & 1, &bars.dead)) break;

@@ -1,6 +1,6 @@
-// attn_rows.cuh -- attention of one query row by one warp, in fp32 on the CUDA cores: the definition written out. Each
-// key is looked at only if the row may see it, so nothing in a masked place (an infinity, a NaN, memory never written)
-// can reach the result.
+// attn_rows.cuh -- attention of one query row by one warp, in fp32 on the CUDA cores: the definition written out, for the
+// rows that the tile kernels must not answer. A key is looked at only if the row may see it, so nothing in a masked place
+// (an infinity, a NaN, memory never written) can reach the result.
 //   s_j = scale (q . k_j),  m = max s_j,  p_j = 2^((s_j - m) log2 e),  out = sum_j p_j v_j / sum_j p_j
 // with the running maximum: one pass over the keys, o and l rescaled when m grows. Lane i holds values
 // [i D / 32, (i + 1) D / 32) of q, o and of every k and v row.
@@ -76,24 +76,55 @@ __device__ __forceinline__ float warp_dot(const float (&a)[N], const float (&b)[
     return s;
 }
 
-// Row of a prompt: query q, keys k0 + j k_stride, j < n; `mine` says which lanes write
+// Row of a prompt whose values in `out` came out non-finite and may owe that to keys the row does not see: query q, keys
+// k0 + j k_stride, j < n. Lanes in `mine` look after their columns: the row is written anew unless all of its NaN turn out to
+// be its own (found as soon as the keys that cause them have been met, so that inputs full of NaN do not cost a pass over
+// all keys per row).
 template <int D, typename T>
-__device__ void attn_row_prompt(const T* q, const T* k0, const T* v0, long long k_stride, long long v_stride, int n, float scale2,
-                                T* out, unsigned mine) {
+__device__ void attn_row_again(const T* q, const T* k0, const T* v0, long long k_stride, long long v_stride, int n, float scale2,
+                               T* out, unsigned mine) {
     constexpr int N = D / 32;
-    const int c = (threadIdx.x & 31) * N;
-    float qv[N], kv[N], vv[N];
+    const int lane = threadIdx.x & 31, c = lane * N;
+    const bool write = mine >> lane & 1;
+    float qv[N], kv[N], vv[N], was[N];
     load_vals(q + c, qv);
+    load_vals(out + c, was);
     RowSoftmax<N> st;
     for (int j = 0; j < n; ++j) {
         load_vals(k0 + j * k_stride + c, kv);
         load_vals(v0 + j * v_stride + c, vv);
         st.key(warp_dot(qv, kv) * scale2, vv);
+        if ((j & 15) == 0) {
+            bool open = false;      // a column of the row that is non-finite for a reason not yet met
+#pragma unroll
+            for (int i = 0; i < N; ++i) open |= !(fabsf(was[i]) < INFINITY) && st.o[i] == st.o[i] && st.l == st.l;
+            if (!__any_sync(0xffffffffu, write && open)) return;
+        }
     }
     const float r = st.l > 0.0f ? 1.0f / st.l : (st.l == 0.0f ? 0.0f : st.l);
 #pragma unroll
     for (int i = 0; i < N; ++i) st.o[i] *= r;
-    if (mine >> (threadIdx.x & 31) & 1) store_vals(out + c, st.o);
+    if (write) store_vals(out + c, st.o);
+}
+
+// Bit r of word r / 32: row r of a tile of 128 (of which `rows` exist) holds a value that is not finite
+template <int D, typename T>
+__device__ __forceinline__ void find_non_finite(const T* v, long long stride, int rows, unsigned (&bits)[4]) {
+    constexpr int N = D / 32;
+    const int c = (threadIdx.x & 31) * N;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        unsigned b = 0;
+        for (int r = 0; r < 32 && w * 32 + r < rows; ++r) {
+            float x[N];
+            load_vals(v + (w * 32 + r) * stride + c, x);
+            bool bad = false;
+#pragma unroll
+            for (int i = 0; i < N; ++i) bad |= !(fabsf(x[i]) < INFINITY);
+            if (__any_sync(0xffffffffu, bad)) b |= 1u << r;
+        }
+        bits[w] = b;
+    }
 }
 
 }  // namespace b200

@@ -77,7 +77,7 @@ def test_pages(lib):
             assert call(s(**ok)) == NODEV, ok
         for bad in (dict(table=None), dict(lens=None), dict(refs=None), dict(info=None), dict(work=None), dict(pool=None),
                     dict(pool=0x10004), dict(n_seqs=0), dict(max_pages=0), dict(n_pages=0), dict(page_shift=-1),
-                    dict(page_shift=27), dict(page_bytes=0), dict(page_bytes=24), dict(n_parts=0), dict(n_parts=2, part_stride=4096),
+                    dict(page_shift=27), dict(n_seqs=1 << 20, max_pages=1 << 12), dict(page_bytes=0), dict(page_bytes=24), dict(n_parts=0), dict(n_parts=2, part_stride=4096),
                     dict(n_parts=2, part_stride=30 * 4096 + 8)):
             assert call(s(**bad)) == BAD, bad
     assert lib.gpu_kv_pages_fork(None, L, None) == BAD

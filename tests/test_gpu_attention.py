@@ -140,6 +140,44 @@ def test_prompt_later_rows_cannot_reach_earlier_ones(ops, D, dt, bad):
     assert torch.isfinite(clean).all()
 
 
+@pytest.mark.parametrize("D,n_q,n_kv,T", [(64, 4, 2, 1500), (128, 2, 2, 1300), (128, 10, 2, 5000), (128, 16, 8, 6000), (256, 4, 1, 1500)])
+def test_prompt_full_of_nan(ops, D, n_q, n_kv, T):
+    """Whole columns, whole tensors and single entries of NaN: what a row sees decides, and it does not take a pass over all
+    keys for every row."""
+    q, k, v, starts, ss = prompt_inputs([T], n_q, n_kv, D, BF, 12)
+    out = torch.empty_like(q)
+    clean = torch.empty_like(q)
+    ops.gpu_attn_prompt(q, k, v, clean, None, 1, T, n_q, n_kv, D, 0.1)
+    run = lambda: ops.gpu_attn_prompt(q, k, v, out, None, 1, T, n_q, n_kv, D, 0.1)  # noqa: E731
+    col = out.view(T, n_q, D)
+    keep = v.clone()
+    v[:, 5] = float("nan")                      # one column of the first key head
+    run()
+    G = n_q // n_kv
+    assert col[:, :G, 5].isnan().all()
+    rest = torch.ones(n_q, D, dtype=torch.bool, device="cuda")
+    rest[:G, 5] = False
+    assert torch.equal(col[:, rest], clean.view(T, n_q, D)[:, rest])
+    v.copy_(keep)
+    v[700, 3] = float("nan")                    # one entry: later rows' column only
+    run()
+    prompt_check(q[:700, :D], k[:700, :D], keep[:700, :D], out[:700, :D], [0, 700], 1, 1, D, 0.1, BF)
+    assert col[700:, :G, 3].isnan().all() and torch.isfinite(col[700:, :G, :3]).all() and torch.isfinite(col[:700]).all()
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    v.fill_(float("nan"))
+    a.record()
+    run()
+    b.record()
+    torch.cuda.synchronize()
+    assert out.isnan().all()
+    v.copy_(keep)
+    k[T // 2] = float("nan")
+    run()
+    torch.cuda.synchronize()
+    assert torch.isfinite(out[:T // 2]).all() and out[T // 2:].isnan().all()
+    assert a.elapsed_time(b) < 1000
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_prompt_large_scores(ops, D):
     """Scores that grow along the sequence by far more than an exponential's range, and fall again."""
@@ -275,7 +313,26 @@ def test_decode_ids_outside_the_cache_are_not_seen(ops, prefix):
     assert torch.isfinite(out).all()
 
 
-def test_two_devices_streams_and_graph(ops):
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_decode_contiguous_cache(ops, D, dt):
+    """kv_shift 30: one page per sequence, memory up to its rows only."""
+    n_q, n_kv, ctx = 4, 2, 333
+    lens = [333, 7, 0, 300]
+    kv = n_kv * D
+    K, V = (torch.randn(4, ctx, kv, generator=torch.Generator(device="cuda").manual_seed(s), device="cuda").to(F16) for s in (1, 2))
+    q = torch.randn(4, n_q * D, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda").to(dt)
+    table = torch.arange(4, dtype=torch.int32, device="cuda").view(4, 1)
+    L, out = torch.tensor(lens, dtype=torch.int32, device="cuda"), torch.empty_like(q)
+    ops.gpu_attn_decode(q, K, V, kv, 30, ctx * kv, 4, table, 1, L, 0, out, n_q, n_kv, D, 4, 0.1)
+    pool = torch.stack([K, V], 1)
+    decode_check(out, q, pool, table, L, 1 << 30, n_q, n_kv, D, 0.1)
+    # one sequence, as the framework's single-sequence cache lies
+    ops.gpu_attn_decode(q[3:], K[3], V[3], kv, 30, 0, 1, table[:1], 1, L[3:], 0, out[3:], n_q, n_kv, D, 1, 0.1)
+    decode_check(out[3:], q[3:], pool[3:], table[:1], L[3:], 1 << 30, n_q, n_kv, D, 0.1)
+
+
+def test_side_stream_and_graph(ops):
     """Side stream, and a captured run replayed on new inputs."""
     lens, n_q, n_kv, D, page, prefix = [300, 400, 500], 8, 2, 128, 16, 256
     pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 7)
