@@ -138,6 +138,7 @@ class Both:
 
 @pytest.mark.parametrize("n_seqs,max_pages,n_pages,shift,words,parts", [
     (1, 1, 1, 0, 4, 1), (3, 4, 9, 4, 12, 1), (7, 6, 40, 2, 8, 3), (40, 20, 300, 4, 5000, 1), (33, 40, 5000, 3, 4, 2), (1500, 3, 4100, 1, 4, 1),
+    (300, 64, 9000, 2, 4, 1), (5, 30, 17001, 2, 8, 2),     # (more than one CTA's worth of table, of pages)
 ])
 def test_random_calls(ops, n_seqs, max_pages, n_pages, shift, words, parts):
     r = random.Random(n_seqs)
@@ -225,3 +226,84 @@ def test_more_slots_than_room(ops):
     ops.gpu_kv_pages_resize(x.h, x.t([9, 5]), slots[:10])
     assert slots.tolist() == want[:10] + [-7] * 10
     x.same()
+
+
+def test_serving_run(ops):
+    """What the calls are for, in the order a serving loop makes them: pages for two prompts, their rows normed, rotated and
+    stored, attention over the prompts; samples forked from them; tokens decoded with and without the shared prefix; the
+    longest prompt freed, the cache compacted, and the next token again. Every attention against 64 bits."""
+    from test_gpu_attention import attend, check
+    n_q, n_kv, D, shift, n_seqs, max_pages, n_pages = 8, 2, 128, 4, 6, 24, 90
+    page, kv, scale, G = 1 << shift, n_kv * D, D ** -0.5, n_q // n_kv
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rnd = lambda *n: torch.randn(*n, generator=g, device="cuda")  # noqa: E731
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool = torch.full((n_pages, 2, page, kv), float("nan"), dtype=torch.float16, device="cuda")
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device="cuda")  # noqa: E731
+    pages = ops.KvPages(torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device="cuda"), z(n_seqs), z(n_pages), z(4), shift, pool,
+                        2 * page * kv * 2)
+    qn, kn = 1 + 0.1 * rnd(D), 1 + 0.1 * rnd(D)
+    history = [(torch.zeros(0, kv, dtype=torch.float16, device="cuda"),) * 2 for _ in range(n_seqs)]
+
+    def rows(positions, slots):
+        """Projections of new tokens -> q, k rows normed and rotated, K / V rows in the cache."""
+        T = len(positions)
+        q, k, v = (rnd(T, w * D).bfloat16() for w in (n_q, n_kv, n_kv))
+        ct, sn = torch.empty(T, D // 2, device="cuda"), torch.empty(T, D // 2, device="cuda")
+        ops.gpu_rope_table(ints(positions), 0, T, D, 0, 1e6, ct, sn)
+        qo, ko = torch.empty_like(q), torch.empty_like(k)
+        ops.gpu_qk_norm_rope_tab(q, k, qn, kn, qo, ko, n_q, n_kv, D, D, ct, sn, T, 1e-6)
+        for i, t in enumerate((ko, v)):
+            ops.gpu_kv_store_f16(t, pool[0, i], kv, slots, 0, T, kv, shift, 2 * page * kv)
+        return qo, ko, v
+
+    def decode(seqs, q, prefix):
+        out = torch.empty_like(q)
+        ops.gpu_attn_decode(q, pool, pool[0, 1], kv, shift, 2 * page * kv, n_pages, pages.table[seqs].contiguous(), max_pages,
+                            pages.lens[seqs].contiguous(), prefix, out, n_q, n_kv, D, len(seqs), scale)
+        for i, s in enumerate(seqs):
+            K, V = history[s]
+            for h in range(n_kv):
+                see = torch.ones(G, K.shape[0], dtype=torch.bool, device="cuda")
+                want, bound = attend(q[i].double().view(n_kv, G, D)[h], K[:, h * D:(h + 1) * D].double(), V[:, h * D:(h + 1) * D].double(), see,
+                                     scale, torch.float16)
+                check(out[i].view(n_kv, G, D)[h], want, bound, torch.bfloat16)
+        return out
+
+    lens = [300, 50]
+    slots = z(350)
+    ops.gpu_kv_pages_resize(pages, ints(lens + [0] * 4), slots)
+    q, k, v = rows(list(range(300)) + list(range(50)), slots)
+    out = torch.empty_like(q)
+    ops.gpu_attn_prompt(q, k, v, out, ints([0, 300, 350]), 2, 350, n_q, n_kv, D, scale)
+    for a, b in ((0, 300), (300, 350)):
+        see = torch.ones(b - a, b - a, dtype=torch.bool, device="cuda").tril()
+        for h in range(n_q):
+            x = slice(h // G * D, h // G * D + D)
+            want, bound = attend(q[a:b, h * D:(h + 1) * D].double(), k[a:b, x].double(), v[a:b, x].double(), see, scale, torch.bfloat16)
+            check(out[a:b, h * D:(h + 1) * D], want, bound, torch.bfloat16)
+    for s, (a, b) in enumerate(((0, 300), (300, 350))):
+        history[s] = (k[a:b].half(), v[a:b].half())
+    ops.gpu_kv_pages_fork(pages, ints([-1, -1, 0, 0, 1, -1]))
+    for s, p in ((2, 0), (3, 0), (4, 1)):
+        history[s] = history[p]
+    assert pages.info.tolist()[:3] == [0, n_pages - 19 - 4 - 3, 3]
+    alive = [0, 1, 2, 3, 4]
+    for step in range(20):
+        now = [history[s][0].shape[0] for s in range(n_seqs)]
+        slots = z(len(alive))
+        ops.gpu_kv_pages_resize(pages, ints([now[s] + 1 if s in alive else -1 for s in range(n_seqs)]), slots)
+        q, k, v = rows([now[s] for s in alive], slots)
+        for i, s in enumerate(alive):
+            history[s] = tuple(torch.cat([x, t[i:i + 1].half()]) for x, t in zip(history[s], (k, v)))
+        if step % 6 == 0:
+            decode(alive, q, 0)
+            decode([0, 2, 3], q[[0, 2, 3]].contiguous(), 288)
+    last = decode([2, 3, 4], q[[2, 3, 4]].contiguous(), 0)
+    ops.gpu_kv_pages_resize(pages, ints([0, 0, -1, -1, -1, -1]))
+    before = pages.refs.clone()
+    ops.gpu_kv_pages_compact(pages)
+    n_live = int((before > 0).sum())
+    assert pages.info.tolist()[:2] == [0, n_pages - n_live] and (pages.refs[:n_live] > 0).all() and (pages.refs[n_live:] == 0).all()
+    assert torch.equal(decode([2, 3, 4], q[[2, 3, 4]].contiguous(), 0), last)
+    decode([2, 3], q[[2, 3]].contiguous(), 288)
