@@ -261,14 +261,10 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 for (int c = 0; c < CW; c += 32) {
                     uint32_t o[32], o1[MODE == BY_KEYS ? 32 : 1];
                     tmem_ld32(o_addr + c0 + c, o);
-                    if constexpr (MODE == BY_KEYS) {
-                        if (tiles > 1) tmem_ld32(o_addr + D + c0 + c, o1);
-                    }
+                    if constexpr (MODE == BY_KEYS) tmem_ld32(o_addr + D + c0 + c, o1);   // (of a single tile: anything)
                     tmem_ld_wait();
                     tmem_pin(o);
-                    if constexpr (MODE == BY_KEYS) {
-                        if (tiles > 1) tmem_pin(o1);
-                    }
+                    if constexpr (MODE == BY_KEYS) tmem_pin(o1);
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         float y[8];
@@ -276,7 +272,8 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                         for (int t = 0; t < 8; ++t) {
                             y[t] = __uint_as_float(o[e + t]) * w0;
                             if constexpr (MODE == BY_KEYS) {
-                                if (tiles > 1) y[t] = fmaf(__uint_as_float(o1[e + t]), w1, y[t]);
+                                const float both = fmaf(__uint_as_float(o1[e + t]), w1, y[t]);
+                                y[t] = tiles > 1 ? both : y[t];
                             }
                             bad |= !(fabsf(y[t]) < INFINITY);
                         }
