@@ -95,14 +95,14 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
         k_stride % 8 || v_stride % 8 || !al16(q) || !al16(k) || !al16(v) || !al16(out) || out == q || out == k || out == v)
         return cudaErrorInvalidValue;
     // How a CTA's two query tiles come about (attn_prompt.cuh): two heads of an even group, else 256 rows; and, where those
-    // are fewer blocks than SMs, one tile whose keys are shared between the two: half the steps for the block that takes
-    // longest, for twice the K and V bytes a step (one sequence of 512 and 1,024 rows, 16 / 8 heads of 128: 12.8 -> 10.1 and
-    // 19.1 -> 14.4 us; at 152 blocks, 2,427 rows, 40.3 -> 40.0 in bf16 and 40.4 -> 50.9 in fp16)
+    // would hardly fill the SMs once, one tile whose keys are shared between the two: half the steps for the block that takes
+    // longest, for twice the K and V bytes a step (one sequence, 16 / 8 heads of 128: 512 rows, 32 blocks, 12.8 -> 9.9 us;
+    // 1,024 rows, 64, 19.1 -> 13.7; 2,427 rows, 152, 39.8 -> 37.4; four of 1,024 rows, heads of 64, 288 blocks: 33 -> 42)
     const int slots128 = (int)(seq_start ? rows / TILE_ROWS + n_seqs : (rows + TILE_ROWS - 1) / TILE_ROWS);
     const long long slots256 = seq_start ? rows / (2 * TILE_ROWS) + n_seqs : (rows + 2 * TILE_ROWS - 1) / (2 * TILE_ROWS);
     const bool even = n_q / n_kv % 2 == 0;
     int mode = D == 256 ? BY_ROWS : even ? BY_HEADS : BY_ROWS;
-    if (D < 256 && (even ? (long long)slots128 * (n_q / 2) : slots256 * n_q) < sm_count()) mode = BY_KEYS;
+    if (D < 256 && (even ? (long long)slots128 * (n_q / 2) : slots256 * n_q) * 4 < 5LL * sm_count()) mode = BY_KEYS;
     const long long n_slots = D < 256 && mode == BY_ROWS ? slots256 : slots128, grid = n_slots * (mode == BY_HEADS ? n_q / 2 : n_q);
     if (grid > INT_MAX) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
@@ -198,6 +198,7 @@ template <int D, typename T>
 cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, int n_q, int n_kv, int B, float scale2, char* scratch,
                             const DecodePlan& pl, cudaStream_t stream) {
     constexpr bool SPLIT = sizeof(T) == 4;
+    const OwnPlan own(n_q, n_kv, OwnShape<D>::WARPS);
     const OwnScratch sc{reinterpret_cast<int*>(scratch), reinterpret_cast<int*>(scratch + pl.first),
                         reinterpret_cast<float*>(scratch + pl.own_ml), reinterpret_cast<float*>(scratch + pl.own_o)};
     // The copy engine takes the cache apart where pages are whole swizzle atoms (8 rows) and a tensor map can describe it;
@@ -216,7 +217,7 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
         static std::atomic<unsigned long long> done;                                                                         \
         if ((st = allow_smem(k_attn_own<D, T, BOX_>, OwnShape<D>::SMEM, done)) != cudaSuccess) return st;                         \
         launch_pdl((k_attn_own<D, T, BOX_>), (unsigned)pl.grid_own, OwnShape<D>::WARPS * 32, OwnShape<D>::SMEM, stream, ok, ov, q, kv, \
-                   sc, n_q, n_kv, B, behind, scale2, 2);                                                                     \
+                   sc, own, n_q, n_q / n_kv, B, behind, scale2, 2);                                                                    \
     } while (0)
     if (box) OWN(true); else OWN(false);
 #undef OWN
@@ -239,7 +240,8 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
 #undef PREFIX
         if ((st = launched()) != cudaSuccess) return st;
     }
-    launch_pdl((k_attn_join<D, T>), (unsigned)(((long long)B * n_q + 3) / 4), 128, 0, stream, kv, sc, px, out, n_q, n_kv, B, behind);
+    launch_pdl((k_attn_join<D, T>), (unsigned)(((long long)B * n_q + 3) / 4), 128, 0, stream, kv, sc, own, px, out, n_q, n_kv,
+               B, behind);
     return launched();
 }
 
@@ -264,10 +266,6 @@ cudaError_t launch_decode(const T* q, const uint16_t* K, const uint16_t* V, int 
 }
 
 // ---------------------------------------------------------------- pages
-
-#ifndef COPY_PER_SM
-#define COPY_PER_SM 8
-#endif
 
 bool good_pages(const b200_kv_pages* kv) {
     return kv && kv->table && kv->lens && kv->refs && kv->info && kv->work && kv->pool && kv->n_seqs > 0 && kv->max_pages > 0 &&
@@ -299,7 +297,7 @@ cudaError_t launch_pages(const b200_kv_pages* kv, cudaStream_t stream, void (*ke
     (void)cudaLaunchKernelEx(&cfg, kernel, static_cast<KA>(args)...);
     const cudaError_t st = launched();
     if (st != cudaSuccess) return st;
-    launch_pdl(k_kv_pages_copy, (unsigned)(sm_count() * COPY_PER_SM), 256, 0, stream, *kv);
+    launch_pdl(k_kv_pages_copy, (unsigned)resident_ctas(256), 256, 0, stream, *kv);
     return launched();
 }
 

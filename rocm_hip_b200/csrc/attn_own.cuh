@@ -18,6 +18,8 @@
 #ifndef B200_ATTN_OWN_CUH
 #define B200_ATTN_OWN_CUH
 
+#include <limits.h>
+
 #include "attn_decode.cuh"
 #include "attn_tiles.cuh"
 
@@ -38,7 +40,7 @@ struct OwnShape {
 // where that leaves warps over, R row groups of 16 run side by side.
 struct OwnPlan {
     int gt, units, groups, wh, R, hg;     // tiles of 8 query heads per key head; units; CTA-sized groups of them; units per CTA
-    __host__ __device__ OwnPlan(int n_q, int n_kv, int warps) {
+    OwnPlan(int n_q, int n_kv, int warps) {
         const int G = n_q / n_kv;
         gt = (G + 7) / 8;
         hg = G < 8 ? G : 8;               // query heads a unit writes at most
@@ -101,7 +103,8 @@ __device__ __forceinline__ int own_rows(const PagedKv& kv, int b, int prefix, in
 // tensor map cannot describe.
 template <int D, typename QT, bool BOX>
 __global__ void __launch_bounds__(OwnShape<D>::WARPS * 32, 1)
-k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const QT* q, PagedKv kv, OwnScratch sc, int n_q, int n_kv, int B, int prefix, float scale2, int min_tiles) {
+k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const QT* q, PagedKv kv, OwnScratch sc, OwnPlan pl, int n_q, int G, int B, int prefix,
+           float scale2, int min_tiles) {
     using Sh = OwnShape<D>;
     constexpr bool SPLIT = sizeof(QT) == 4;
     constexpr int W = Sh::WARPS, ST = Sh::STAGES, KS = D / 16, UNITS = D / 8, NT = W * 32;
@@ -117,8 +120,7 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
         tma_prefetch(&mv);
     }
     pdl_entry();
-    const OwnPlan pl(n_q, n_kv, W);
-    const int G = n_q / n_kv, tile = 16 * pl.R;
+    const int tile = 16 * pl.R;
 
     // ---- the shares: every CTA sums the tiles of all sequences, then finds where its own share begins
     const auto tiles_of = [&](int b) {
@@ -418,20 +420,32 @@ struct PrefixScratch {
 // cover; a row without pieces, or with none that saw a key, is zero. A warp per row.
 template <int D, typename QT>
 __global__ void __launch_bounds__(128)
-k_attn_join(PagedKv kv, OwnScratch sc, PrefixScratch px, QT* out, int n_q, int n_kv, int B, int prefix) {
+k_attn_join(PagedKv kv, OwnScratch sc, OwnPlan pl, PrefixScratch px, QT* out, int n_q, int n_kv, int B, int prefix) {
     pdl_entry();
     constexpr int N = D / 32, W = OwnShape<D>::WARPS;
-    const long long row = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (row >= (long long)B * n_q) return;
-    const int b = (int)(row / n_q), h = (int)(row % n_q), G = n_q / n_kv, kh = h / G, g = h % G;
-    const OwnPlan pl(n_q, n_kv, W);
-    const int u = kh * pl.gt + g / 8, grp = u / pl.wh, wu = u % pl.wh;
-    const long long per = *reinterpret_cast<const long long*>(sc.head);
-    const int n_tiles = sc.first[b + 1] - sc.first[b];
-    const long long t0 = (long long)sc.first[b] * pl.groups + (long long)grp * n_tiles;
-    const int c0 = n_tiles ? (int)(t0 / per) : 0, n_own = n_tiles ? ((int)((t0 + n_tiles - 1) / per) - c0 + 1) * pl.R : 0;
-    const int n_px = kv.len(b) >= prefix ? px.splits : 0, n = n_px + n_own;
+    const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;     // (B n_q <= 2^28)
+    if (row >= B * n_q) return;
+    const int b = row / n_q, h = row - b * n_q, G = n_q / n_kv, kh = h / G, g = h - kh * G;
+    const int u = kh * pl.gt + g / 8, grp = u / pl.wh, wu = u - grp * pl.wh;
+    // (volatile: all four are under way before the first is needed; left to the compiler, two of them waited for the others)
+    const int before = *(const volatile int*)(sc.first + b), n_tiles = *(const volatile int*)(sc.first + b + 1) - before;
+    const long long per = *(const volatile long long*)sc.head;
+    const int len = *(const volatile int*)(kv.lens + b);
+    const int n_px = (long long)len >= prefix && ((long long)kv.max_pages << kv.kv_shift) >= prefix ? px.splits : 0;
+    const long long t0 = (long long)before * pl.groups + (long long)grp * n_tiles, t1 = t0 + n_tiles - 1;
+    int c0 = 0, n_own = 0;
+    if (n_tiles > 0) {
+        int c1;
+        if (t1 < INT_MAX) {      // (a 64-bit division is a hundred instructions)
+            c0 = (int)t0 / (int)per;
+            c1 = (int)t1 / (int)per;
+        } else {
+            c0 = (int)(t0 / per);
+            c1 = (int)(t1 / per);
+        }
+        n_own = (c1 - c0 + 1) * pl.R;
+    }
+    const int n = n_px + n_own;
     // piece i of the row -> its (m, l) and o
     const auto piece = [&](int i, const float** o) -> const float* {
         if (i < n_px) {
@@ -440,8 +454,9 @@ k_attn_join(PagedKv kv, OwnScratch sc, PrefixScratch px, QT* out, int n_q, int n
             return px.ml + at * 2;
         }
         i -= n_px;
-        const long long slot = c0 + i / pl.R + (long long)b * pl.groups + grp;
-        const long long at = (slot * W + wu + i % pl.R * pl.wh) * pl.hg + g % 8;
+        const int k = pl.R == 1 ? i : i / pl.R;
+        const long long slot = c0 + k + (long long)b * pl.groups + grp;
+        const long long at = (slot * W + wu + (i - k * pl.R) * pl.wh) * pl.hg + g % 8;
         *o = sc.o + at * D;
         return sc.ml + at * 2;
     };
@@ -469,15 +484,16 @@ k_attn_join(PagedKv kv, OwnScratch sc, PrefixScratch px, QT* out, int n_q, int n
 #pragma unroll
         for (int e = 0; e < N; ++e) acc[e] *= old;
         const int count = min(32, n - i0);
-        for (int i = 0; i < count; i += 8) {    // eight rows in flight
-            float v[8][N];
+        constexpr int F = N == 8 ? 8 : 16;       // rows in flight
+        for (int i = 0; i < count; i += F) {
+            float v[F][N];
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
+            for (int t = 0; t < F; ++t) {
                 const float* o = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, (unsigned long long)mine, i + t));
                 if (i + t < count) load_vals(o + lane * N, v[t]);
             }
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
+            for (int t = 0; t < F; ++t) {
                 const float ft = __shfl_sync(0xffffffffu, f, i + t);
                 if (i + t < count)
 #pragma unroll
@@ -488,7 +504,7 @@ k_attn_join(PagedKv kv, OwnScratch sc, PrefixScratch px, QT* out, int n_q, int n
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] *= inv;
-    store_vals(out + row * D + lane * N, acc);
+    store_vals(out + (long long)row * D + lane * N, acc);
 }
 
 }  // namespace b200

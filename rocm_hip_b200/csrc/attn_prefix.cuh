@@ -29,7 +29,7 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
               int n_q, int n_kv, int B, int prefix, float scale2, int row_tiles) {
     constexpr bool SPLIT = sizeof(QT) == 4;
     using Ti = typename PrefixShape<D, NQ, SPLIT>::Ti;
-    constexpr int SC = PrefixShape<D, NQ, SPLIT>::SC, N = D / 32;
+    constexpr int SC = PrefixShape<D, NQ, SPLIT>::SC;
     extern __shared__ unsigned char smem_raw[];
     __shared__ TileBars bars;
     unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -96,40 +96,41 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
     } else if (warp < NQ * 4) {
         Ti::many_registers();
         const int i = warp >> 2, mine = r0 + warp * 32;     // this warp's 32 query rows
-        // ---- queries to shared memory, a row of D values by the whole warp: K-major, 128-byte swizzle
+        // ---- queries to shared memory: four lanes to a row, eight rows at a time; K-major with 128-byte swizzle. (The whole warp
+        // to a row, 32 rows one after another, was 15 us of a stretch's 27: one warp per scheduler issues an instruction every
+        // few clocks, and it took five times as many.)
         float c_row = 0.0f;
-        for (int r8 = 0; r8 < 32; r8 += 8) {      // eight rows in flight
-            float v[8][N], top[8];
+        constexpr int VE = Io<QT>::VE, NV = D / 4 / VE;     // values in 16 bytes, and 16-byte loads of a lane
+#pragma unroll 1
+        for (int r8 = 0; r8 < 32; r8 += 8) {
+            const int r = mine + r8 + (lane >> 2), in_tile = (warp & 3) * 32 + r8 + (lane >> 2);
+            const QT* src = q + ((long long)(r / G) * n_q + kh * G + r % G) * D + (lane & 3) * VE;
+            float v[NV][VE], top = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const int r = mine + r8 + t;
+            for (int k = 0; k < NV; ++k) {
+                const uint4 raw = r < M ? __ldg(reinterpret_cast<const uint4*>(src + k * 4 * VE)) : make_uint4(0, 0, 0, 0);
+                Io<QT>::unpack(raw, v[k]);
 #pragma unroll
-                for (int e = 0; e < N; ++e) v[t][e] = 0.0f;
-                if (r < M) load_vals(q + ((long long)(r / G) * n_q + kh * G + r % G) * D + lane * N, v[t]);
+                for (int e = 0; e < VE; ++e) top = fmaxf(top, fabsf(v[k][e]));
             }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int x = q_exponent(top);
+            const float k0 = pow2(x / 2), k1 = pow2(x - x / 2), c = __shfl_sync(0xffffffffu, scale2e(scale2, -x), (lane & 7) * 4);
+            if (lane >> 3 == r8 >> 3) c_row = c;
+            unsigned char* row = smem + i * Ti::QTILE * (SPLIT ? 2 : 1) + in_tile * 128;
 #pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                top[t] = 0.0f;
+            for (int k = 0; k < NV; ++k) {
+                const int col = (k * 4 + (lane & 3)) * VE;
+                unsigned char* at = row + col / CHUNK * CHUNK_BYTES + ((col % CHUNK / 8 ^ (in_tile & 7)) * 16) + col % 8 * 2;
+                uint32_t hi[VE / 2], lo[VE / 2];
 #pragma unroll
-                for (int e = 0; e < N; ++e) top[t] = fmaxf(top[t], fabsf(v[t][e]));
-            }
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1)
-#pragma unroll
-                for (int t = 0; t < 8; ++t) top[t] = fmaxf(top[t], __shfl_xor_sync(0xffffffffu, top[t], off));
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                const int x = q_exponent(top[t]);
-                if (lane == r8 + t) c_row = scale2e(scale2, -x);
-                const int col = lane * N, in_tile = (warp & 3) * 32 + r8 + t;
-                unsigned char* at = smem + i * Ti::QTILE * (SPLIT ? 2 : 1) + col / CHUNK * CHUNK_BYTES + in_tile * 128 +
-                                    (((col % CHUNK / 8) ^ (in_tile & 7)) * 16) + col % 8 * 2;
-#pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    uint32_t hi, lo;
-                    split16(scale2e(v[t][e], x), scale2e(v[t][e + 1], x), &hi, &lo);
-                    *reinterpret_cast<uint32_t*>(at + e * 2) = hi;
-                    if constexpr (SPLIT) *reinterpret_cast<uint32_t*>(at + Ti::QTILE + e * 2) = lo;
+                for (int e = 0; e < VE / 2; ++e) split16(v[k][2 * e] * k0 * k1, v[k][2 * e + 1] * k0 * k1, &hi[e], &lo[e]);
+                if constexpr (SPLIT) {
+                    *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+                    *reinterpret_cast<uint2*>(at + Ti::QTILE) = make_uint2(lo[0], lo[1]);
+                } else {
+                    *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[VE / 2 - 2], hi[VE / 2 - 1]);
                 }
             }
         }
