@@ -519,7 +519,7 @@ void b200_gguf_free_tensor(void* dev_ptr);
  * projection. out [T][n_q * head_dim] is contiguous and shares no memory with the inputs. Empty sequences are
  * allowed; rows before the first and behind the last sequence are neither read into a result nor written, and a row's
  * result depends on no k or v that it does not see, non-finite ones included. Weights are
- * rounded to the rows' type before they meet v (the sum of weights is not), out once. T <= 2^30; pointers 16-byte
+ * rounded to the rows' type before they meet v (the sum of weights is not), out once. T <= 2^27; pointers 16-byte
  * aligned. */
 cudaError_t gpu_attn_prompt_bf16(const uint16_t* q, const uint16_t* k, const uint16_t* v, uint16_t* out, const int* seq_start,
                                  int n_seqs, long long T, int n_q, int n_kv, int head_dim, long long q_stride, long long k_stride,

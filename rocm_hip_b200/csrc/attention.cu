@@ -85,7 +85,7 @@ template <typename T>
 cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int* seq_start, int n_seqs, long long rows, int n_q,
                           int n_kv, int D, long long q_stride, long long k_stride, long long v_stride, float scale,
                           cudaStream_t stream) {
-    if (!q || !k || !v || !out || n_seqs < 1 || (!seq_start && n_seqs != 1) || rows < 1 || rows > (1 << 30) ||
+    if (!q || !k || !v || !out || n_seqs < 1 || (!seq_start && n_seqs != 1) || rows < 1 || rows > (1 << 27) ||
         !good_heads(n_q, n_kv, D) || !good_scale(scale))
         return cudaErrorInvalidValue;
     if (q_stride == 0) q_stride = (long long)n_q * D;

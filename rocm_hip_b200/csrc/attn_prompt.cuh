@@ -96,7 +96,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
     unsigned taken = 0;
     const auto next_item = [&](PromptItem* it) {
         const int slot = taken & 1;
-        if (!warp_wait(&pb.item_full[slot], taken >> 1 & 1, &bars.dead)) return false;
+        if (!warp_wait_long(&pb.item_full[slot], taken >> 1 & 1, &bars.dead)) return false;
         *it = pb.item[slot];
         __syncwarp();
         if (lane == 0) mbar_arrive(&pb.item_empty[slot]);
@@ -150,7 +150,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             }
             if (it.n[0] > 0 || block < 0) {
                 const int s = made & 1;
-                if (!warp_wait(&pb.item_empty[s], made >> 1 & 1 ^ 1, &bars.dead)) break;
+                if (!warp_wait_long(&pb.item_empty[s], made >> 1 & 1 ^ 1, &bars.dead)) break;
                 if (lane == 0) {
                     pb.item[s] = it;
                     mbar_arrive(&pb.item_full[s]);

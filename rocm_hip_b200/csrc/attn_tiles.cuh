@@ -50,9 +50,29 @@ __device__ __forceinline__ bool wait_or_die(unsigned long long* bar, unsigned pa
     return false;
 }
 
-// the same for a whole warp: all lanes go on, or none
+// The same for a whole warp: all lanes go on, or none. Such a wait is for one key tile's work of another role, microseconds;
+// MBAR_POLLS are milliseconds at least.
 __device__ __forceinline__ bool warp_wait(unsigned long long* bar, unsigned parity, volatile int* dead) {
     return __all_sync(0xffffffffu, wait_or_die(bar, parity, dead));
+}
+
+// A wait for another role's whole query tile, which takes two microseconds per 128 keys: a look every half microsecond after
+// the first few thousand, for some eight seconds in all
+__device__ __forceinline__ bool warp_wait_long(unsigned long long* bar, unsigned parity, volatile int* dead) {
+    const unsigned b = smem_u32(bar);
+    bool there = false;
+    for (int i = 0; i < (1 << 24) && !there; ++i) {
+        unsigned ok;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(b), "r"(parity)
+                     : "memory");
+        there = ok;
+        if (!there && *dead) break;
+        if (!there && i > 4096) __nanosleep(500);
+    }
+    if (!there) *dead = 1;
+    return __all_sync(0xffffffffu, there);
 }
 
 // SC: columns of a ring stage (a K or V tile is D / SC stages of 128 rows), ST: stages
