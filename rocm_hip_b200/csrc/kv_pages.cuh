@@ -378,9 +378,9 @@ k_kv_pages_compact(b200_kv_pages kv) {
     if (cta == 0 && threadIdx.x == 0) kvp_tell(kv, w.head, KVP_OK, kv.n_pages - n_live, n_move);
 }
 
-// Copies the listed pages, part by part, in tiles of 16 KB: eight CTAs per SM, 64 bytes of each thread's in flight (4,865
+// Copies the listed pages, part by part, in tiles of 16 KB: eight CTAs per SM, 64 bytes of each thread's in flight (4,870
 // pages of 256 KB: 0.42 ms, 6.0 TB/s read and written; two and four CTAs per SM took 2 % longer and 1 % less there, and 9 %
-// and 2 % longer for 300 pages of 1 MB). How many pages there are is known on the device only, so the grid is what fits.
+// and 2 % longer for 320 pages of 1 MB). How many pages there are is known on the device only, so the grid is what fits.
 __global__ void __launch_bounds__(256)
 k_kv_pages_copy(b200_kv_pages kv) {
     pdl_entry();

@@ -75,6 +75,7 @@ def prompt_check(q, k, v, out, starts, n_q, n_kv, D, scale, dt):
 PROMPTS = [
     ([1], 1, 1), ([2], 2, 1), ([127], 2, 2), ([128], 4, 2), ([129], 2, 1), ([255], 5, 1), ([256], 2, 2), ([257], 3, 1), ([700], 2, 1),
     ([1, 1, 1, 1, 1], 2, 1), ([0, 5, 0, 0, 130, 0], 4, 2), ([17, 300, 1, 128, 64, 513], 10, 2), ([1100, 3], 1, 1),
+    ([(i * 37) % 11 for i in range(150)], 2, 1), ([260, 0, 300, 20] * 10, 6, 2),
 ]
 
 
@@ -252,6 +253,8 @@ DECODES = [   # lens, n_q, n_kv, page, prefix
     ([1], 1, 1, 16, 0), ([0], 2, 1, 16, 0), ([5, 0, 77, 64, 65], 4, 2, 16, 0), ([300] * 3, 5, 1, 8, 0), ([1000, 1, 513], 16, 2, 128, 0),
     ([128, 129, 0, 191], 4, 2, 64, 128), ([256 + i * 7 for i in range(9)], 10, 2, 32, 256), ([2048, 2100, 100, 2049], 8, 1, 16, 2048),
     ([700 + 13 * i for i in range(33)], 2, 2, 16, 688), ([1024 + i for i in range(70)], 8, 2, 256, 1024), ([40, 41, 55], 3, 1, 1, 40),
+    ([9, 300, 77, 0, 64], 12, 12, 16, 0), ([350, 400, 266], 9, 3, 16, 256), ([310, 288, 500], 32, 16, 8, 288),
+    ([(7 * i) % 90 for i in range(600)], 2, 2, 16, 0), ([256 + (i % 40) for i in range(300)], 1, 1, 64, 256),
     ([500, 600], 40, 2, 4, 400), ([130], 17, 1, 2, 128), ([3000 + 50 * i for i in range(20)], 20, 4, 64, 2944),
 ]
 
@@ -332,6 +335,75 @@ def test_decode_contiguous_cache(ops, D, dt):
     decode_check(out[3:], q[3:], pool[3:], table[:1], L[3:], 1 << 30, n_q, n_kv, D, 0.1)
 
 
+@pytest.mark.parametrize("page", [4, 64])
+def test_decode_offsets_beyond_32_bits(ops, page):
+    """Pages that begin more than 2^32 values into the cache."""
+    n_q, n_kv, D = 4, 2, 128
+    kv = n_kv * D
+    n_pages = (2**32 + 2**30) // (2 * page * kv)
+    pool = torch.empty(n_pages, 2, page, kv, dtype=F16, device="cuda")
+    lens = [300, 290, 0, 310]
+    shared = 256 // page
+    ids = list(range(n_pages - 1, n_pages - 1 - shared, -1))
+    table = torch.full((4, 400 // page + 2), -1, dtype=torch.int32)
+    at = n_pages - shared - 1
+    for b, n in enumerate(lens):
+        mine = -(-n // page) - shared if n else 0
+        row = (ids if n else []) + list(range(at, at - mine, -1))
+        at -= mine
+        table[b, :len(row)] = torch.tensor(row, dtype=torch.int32)
+    assert at * 2 * page * kv > 2**32
+    pool[at:] = torch.randn(n_pages - at, 2, page, kv, device="cuda").to(F16)
+    L, table = torch.tensor(lens, dtype=torch.int32, device="cuda"), table.cuda()
+    q = torch.randn(4, n_q * D, device="cuda")
+    for prefix in (0, 256):
+        out = decode(ops, q, pool, table, L, kv, n_pages, table.shape[1], page, prefix, n_q, n_kv, D, 0.1)
+        decode_check(out, q, pool, table, L, page, n_q, n_kv, D, 0.1)
+
+
+def test_prompt_offsets_beyond_32_bits(ops):
+    """Rows that begin more than 2^31 values into q and out, at the end of a long batch of short prompts."""
+    n_q, n_kv, D, n = 64, 2, 128, 100
+    seqs = 2**31 // (n_q * D * n) + 3
+    T = seqs * n
+    q = torch.empty(T, n_q * D, dtype=BF, device="cuda").normal_()
+    k, v = (torch.randn(T, n_kv * D, device="cuda").to(BF) for _ in range(2))
+    out = torch.empty_like(q)
+    ss = torch.arange(seqs + 1, dtype=torch.int32, device="cuda") * n
+    ops.gpu_attn_prompt(q, k, v, out, ss, seqs, T, n_q, n_kv, D, 0.1)
+    for b in (0, seqs - 2, seqs - 1):
+        a = b * n
+        prompt_check(q[a:a + n], k[a:a + n], v[a:a + n], out[a:a + n], [0, n], n_q, n_kv, D, 0.1, BF)
+
+
+def test_calls_at_once(ops):
+    """The same work on two streams at a time, each with its own scratch: every result as alone."""
+    sets = []
+    for seed in range(2):
+        pool, table, L, stride, n_pages, max_pages = paged([600 + 40 * i for i in range(9)], 2, 128, 16, 512, seed)
+        q = torch.randn(9, 8 * 128, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(BF if seed else F32)
+        qp, k, v, _, ss = prompt_inputs([700, 90, 333], 4, 2, 64 if seed else 128, BF, seed)
+        sets.append((pool, table, L, stride, n_pages, max_pages, q, qp, k, v, ss, torch.cuda.Stream()))
+
+    def work(s):
+        pool, table, L, stride, n_pages, max_pages, q, qp, k, v, ss, _ = s
+        out = decode(ops, q, pool, table, L, stride, n_pages, max_pages, 16, 512, 8, 2, 128, 0.1)
+        po = torch.zeros_like(qp)
+        ops.gpu_attn_prompt(qp, k, v, po, ss, 3, qp.shape[0], 4, 2, qp.shape[1] // 4, 0.1)
+        return out, po
+
+    alone = [work(s) for s in sets]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        got = []
+        for s in sets:
+            with torch.cuda.stream(s[-1]):
+                got.append(work(s))
+        torch.cuda.synchronize()
+        for a, b in zip(alone, got):
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
 def test_side_stream_and_graph(ops):
     """Side stream, and a captured run replayed on new inputs."""
     lens, n_q, n_kv, D, page, prefix = [300, 400, 500], 8, 2, 128, 16, 256
@@ -373,5 +445,13 @@ def test_types_are_checked(ops):
         ops.gpu_attn_prompt(x, x, x, x.clone(), None, 1, 4, 1, 1, 128, 0.1)
     with pytest.raises(TypeError):
         ops.gpu_attn_prompt(h, h.to(F16), h, h.clone(), None, 1, 4, 1, 1, 128, 0.1)
+    with pytest.raises(ValueError):      # not on the current device
+        ops.gpu_attn_prompt(h.cpu(), h, h, h.clone(), None, 1, 4, 1, 1, 128, 0.1)
     with pytest.raises(ops.LayerOpError):
         ops.gpu_attn_prompt(h, h, h, h, None, 1, 4, 1, 1, 128, 0.1)
+
+
+def test_no_block_gave_up(ops):
+    """Collected last: none of the waits of the tests before has run out."""
+    from rocm_hip_b200 import _lib
+    assert _lib.load().b200_attn_gave_up() == 0
