@@ -98,11 +98,11 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
     // would hardly fill the SMs once, one tile whose keys are shared between the two: half the steps for the block that takes
     // longest, for twice the K and V bytes a step (one sequence, 16 / 8 heads of 128: 512 rows, 32 blocks, 12.8 -> 9.9 us;
     // 1,024 rows, 64, 19.1 -> 13.7; 2,427 rows, 152, 39.8 -> 37.4; four of 1,024 rows, heads of 64, 288 blocks: 33 -> 42)
-    const int slots128 = (int)(seq_start ? rows / TILE_ROWS + n_seqs : (rows + TILE_ROWS - 1) / TILE_ROWS);
+    const long long slots128 = seq_start ? rows / TILE_ROWS + n_seqs : (rows + TILE_ROWS - 1) / TILE_ROWS;
     const long long slots256 = seq_start ? rows / (2 * TILE_ROWS) + n_seqs : (rows + 2 * TILE_ROWS - 1) / (2 * TILE_ROWS);
     const bool even = n_q / n_kv % 2 == 0;
     int mode = D == 256 ? BY_ROWS : even ? BY_HEADS : BY_ROWS;
-    if (D < 256 && (even ? (long long)slots128 * (n_q / 2) : slots256 * n_q) * 4 < 5LL * sm_count()) mode = BY_KEYS;
+    if (D < 256 && (even ? slots128 * (n_q / 2) : slots256 * n_q) * 4 < 5LL * sm_count()) mode = BY_KEYS;
     const long long n_slots = D < 256 && mode == BY_ROWS ? slots256 : slots128, grid = n_slots * (mode == BY_HEADS ? n_q / 2 : n_q);
     if (grid > INT_MAX) return cudaErrorInvalidValue;
     if (!lib_ready()) return cudaErrorInvalidDeviceFunction;
@@ -207,7 +207,9 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
     // cache is one of 2^30) need not be memory up to there.
     CUtensorMap mk, mv, ok, ov;
     const bool box = kv.kv_shift >= 3 && kv.kv_shift <= 12 && page_map(&ok, kv.K, D, n_kv, kv, 16) && page_map(&ov, kv.V, D, n_kv, kv, 16);
-    const bool shared = pl.splits > 0 && kv.kv_shift >= 3 && page_map(&mk, kv.K, D, n_kv, kv, TILE_ROWS) && page_map(&mv, kv.V, D, n_kv, kv, TILE_ROWS);
+    const long long grid = (long long)n_kv * pl.row_tiles * pl.splits;
+    const bool shared = grid > 0 && grid <= INT_MAX && kv.kv_shift >= 3 && page_map(&mk, kv.K, D, n_kv, kv, TILE_ROWS) &&
+                        page_map(&mv, kv.V, D, n_kv, kv, TILE_ROWS);
     const PrefixScratch px{shared ? pl.splits : 0, pl.px_rows, reinterpret_cast<float*>(scratch + pl.px_ml),
                            reinterpret_cast<float*>(scratch + pl.px_o)};
     const int behind = shared ? prefix : 0;
@@ -223,13 +225,12 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
 #undef OWN
     if ((st = launched()) != cudaSuccess) return st;
     if (shared) {
-        const unsigned grid = (unsigned)((long long)n_kv * pl.row_tiles * pl.splits);
 #define PREFIX(NQ_)                                                                                                       \
     do {                                                                                                                  \
         using Ti = typename PrefixShape<D, NQ_, SPLIT>::Ti;                                                               \
         static std::atomic<unsigned long long> done;                                                                      \
         if ((st = allow_smem(k_attn_prefix<D, NQ_, T>, Ti::SMEM, done)) != cudaSuccess) return st;                             \
-        launch_pdl((k_attn_prefix<D, NQ_, T>), grid, Ti::WARPS * 32, Ti::SMEM, stream, mk, mv, q, kv, px, n_q, n_kv, B, prefix, scale2, \
+        launch_pdl((k_attn_prefix<D, NQ_, T>), (unsigned)grid, Ti::WARPS * 32, Ti::SMEM, stream, mk, mv, q, kv, px, n_q, n_kv, B, prefix, scale2, \
                    pl.row_tiles);                                                                                         \
     } while (0)
         if constexpr (D < 256) {

@@ -6,6 +6,8 @@
 #ifndef B200_ATTN_DECODE_CUH
 #define B200_ATTN_DECODE_CUH
 
+#include <limits.h>
+
 #include "attn_rows.cuh"
 #include "kv_store.cuh"
 
@@ -18,9 +20,9 @@ struct PagedKv {
     const int* lens;    // [B]
     long long kv_bstride;
     int kv_stride, kv_shift, n_pages, max_pages;
-    // rows of sequence b: lens[b] within what its page list can hold
+    // rows of sequence b: lens[b] within what its page list can hold (and a little below 2^31, so that whole tiles fit an int)
     __device__ __forceinline__ int len(int b) const {
-        const long long cap = (long long)max_pages << kv_shift;
+        const long long cap = min((long long)max_pages << kv_shift, (long long)INT_MAX - 4096);
         const long long n = max(lens[b], 0);
         return (int)(n < cap ? n : cap);
     }

@@ -103,8 +103,8 @@ __device__ __forceinline__ int own_rows(const PagedKv& kv, int b, int prefix, in
 // tensor map cannot describe.
 template <int D, typename QT, bool BOX>
 __global__ void __launch_bounds__(OwnShape<D>::WARPS * 32, 1)
-k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const QT* q, PagedKv kv, OwnScratch sc, OwnPlan pl, int n_q, int G, int B, int prefix,
-           float scale2, int min_tiles) {
+k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv, const QT* q, PagedKv kv, OwnScratch sc,
+           OwnPlan pl, int n_q, int G, int B, int prefix, float scale2, int min_tiles) {
     using Sh = OwnShape<D>;
     constexpr bool SPLIT = sizeof(QT) == 4;
     constexpr int W = Sh::WARPS, ST = Sh::STAGES, KS = D / 16, UNITS = D / 8, NT = W * 32;

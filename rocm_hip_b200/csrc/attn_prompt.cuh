@@ -57,7 +57,7 @@ __device__ __forceinline__ int block_answer(PromptBars& pb) {   // the block's i
 // The grid is all blocks of work, heaviest first as far as one pass over the batch knows; a CTA that has finished one takes
 // the next that nobody has begun. Its roles run ahead of one another: while the softmax warps still write one block's rows,
 // the schedule warp has looked up the next block, its first K and V tiles are on their way, and the tensor cores begin as
-// soon as the last scores against the query tile are done. (One CTA per block: 61 sequences of 200 rows, 16 heads of 64, took 98 us, most of
+// soon as the query tile's memory is free and filled again. (One CTA per block: 61 sequences of 200 rows, 16 heads of 64, took 98 us, most of
 // it the way from a CTA's start to its first product and from its last to its end.)
 template <int D, typename T, int MODE>
 __global__ void __launch_bounds__(PromptTiles<D, T>::WARPS * 32, 1)

@@ -92,8 +92,8 @@ struct Tiles {
     static constexpr int P_SHIFT_T = std::is_same<T, __half>::value ? 7 : 0;   // fp16 weights are held times 2^7 (at most 2^15)
 
     // A softmax thread holds its row's 128 scores: 224 registers. Twelve warps start with 168 each (64,512 in all); the four
-    // that compute nothing go down to 56 and the eight softmax warps up, 4 x 32 x 56 + 8 x 32 x 224 = 64,512. (Six warps
-    // may have 255 from the start.)
+    // that compute nothing go down to 56 and the eight softmax warps up, 4 x 32 x 56 + 8 x 32 x 224 = 64,512. (Seven
+    // warps may have 255 from the start.)
     static __device__ __forceinline__ void few_registers() {
         if constexpr (NQ == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     }

@@ -35,7 +35,7 @@ def test_prompt(lib, name):
                dict(q_stride=1536, k_stride=1536, v_stride=1536), dict(T=1), dict(n_seqs=1000), dict(n_q=10)):
         assert call(**ok) == NODEV, ok
     for bad in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(seq_start=None), dict(n_seqs=0), dict(T=0), dict(T=-1),
-                dict(T=(1 << 27) + 1), dict(n_q=7), dict(n_q=0), dict(n_kv=0), dict(n_kv=-2), dict(head_dim=96), dict(head_dim=512),
+                dict(T=(1 << 27) + 1), dict(n_seqs=2**31 - 1), dict(n_q=7), dict(n_q=0), dict(n_kv=0), dict(n_kv=-2), dict(head_dim=96), dict(head_dim=512),
                 dict(head_dim=0), dict(q_stride=1000), dict(q_stride=1020), dict(k_stride=255), dict(v_stride=-256), dict(scale=0.0),
                 dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(out=Q), dict(out=V),
                 dict(q=C.c_void_p(0x10008)), dict(out=C.c_void_p(0x40002))):
