@@ -543,7 +543,8 @@ int b200_attn_gave_up(void);
  * fewer rows (idle slots) use their own pages only. Memory behind lens[b] may hold anything; a page of up to 4096 rows is
  * readable to its end, of larger ones (a contiguous cache: kv_shift 30, one page per sequence) nothing behind lens[b] is
  * touched.
- * fp32 rows keep fp32 accuracy; kv_stride and kv_bstride are multiples of 8, pointers 16-byte aligned, out is not q.
+ * fp32 rows come out to a few 1e-6 of the result's norm (two fp16 values a query value and weight). kv_stride and
+ * kv_bstride are multiples of 8, pointers 16-byte aligned, out is not q.
  * scratch: device memory of gpu_attn_decode_scratch_bytes(...) bytes, any contents, in use until the call has run; calls
  * that may overlap need scratch of their own. */
 size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len);

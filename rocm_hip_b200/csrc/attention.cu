@@ -169,8 +169,9 @@ struct DecodePlan {
             // stretches of the prefix: as many as make the CTAs whole waves of the device, counting about four tiles' time
             // for what a CTA does once (its queries, its result and the pieces' way through scratch). For fp32 rows no
             // longer than six tiles: the tensor cores cut sums off where fp32 arithmetic rounds, a stretch of t tiles
-            // (16 t additions) loses 2.5e-8 per addition, and joining stretches does not (8,192 rows, heads of 256: 3.5e-6
-            // with stretches of nine tiles, 2.6e-6 with six; 32,768 rows, heads of 128: 1.1e-5 with 37, 2.5e-6 with six).
+            // (16 t additions) loses up to 2.5e-8 per addition, and joining stretches does not (against 64 bits: 8,192 rows,
+            // heads of 256, 1.7e-6; 32,768 rows, heads of 128, 1.4e-6; stretches of nine and of 37 tiles, which the waves
+            // alone would give, lost twice and eight times as much).
             const int tiles = (prefix + TILE_ROWS - 1) / TILE_ROWS, base = n_kv * row_tiles;
             const int least = f32 ? (tiles + 5) / 6 : 1;
             long long best = LLONG_MAX;

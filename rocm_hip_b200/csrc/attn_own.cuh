@@ -314,21 +314,21 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                         }
                         __syncwarp();
                         // two chains of products, so that one's latency hides the other's
-                        float st[4] = {0.0f, 0.0f, 0.0f, 0.0f}, su[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float st[4] = {0.0f, 0.0f, 0.0f, 0.0f}, su[4] = {0.0f, 0.0f, 0.0f, 0.0f}, sl[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                         for (int i = 0; i < KS; i += 2) {
                             uint32_t a[4], c[4];
                             ldsm4(smem_u32(Kt) + own_at((lane & 7) + (lane >> 3 & 1) * 8, i * 2 + (lane >> 4)), a);
                             ldsm4(smem_u32(Kt) + own_at((lane & 7) + (lane >> 3 & 1) * 8, i * 2 + 2 + (lane >> 4)), c);
                             if constexpr (SPLIT) {
-                                mma16(st, a, ql[i][0], ql[i][1]);
-                                mma16(su, c, ql[i + 1][0], ql[i + 1][1]);
+                                mma16(sl, a, ql[i][0], ql[i][1]);
+                                mma16(sl, c, ql[i + 1][0], ql[i + 1][1]);
                             }
                             mma16(st, a, qh[i][0], qh[i][1]);
                             mma16(su, c, qh[i + 1][0], qh[i + 1][1]);
                         }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) st[i] += su[i];
+                        for (int i = 0; i < 4; ++i) st[i] = (sl[i] + su[i]) + st[i];
                         const bool s0 = seen[s] >> g8 & 1, s1 = seen[s] >> (g8 + 8) & 1;
                         const float x0 = s0 ? st[0] * c0 : -INFINITY, x1 = s0 ? st[1] * c1 : -INFINITY;
                         const float x2 = s1 ? st[2] * c0 : -INFINITY, x3 = s1 ? st[3] * c1 : -INFINITY;

@@ -190,16 +190,16 @@ struct Tiles {
         const auto score = [&](int i, int buf, int stage) {   // S[buf] = Q_i K^T, Q_0 if KEYS
             const uint32_t d = tmem + buf * 128;
             if (elect_one()) {
+                // (SPLIT: the low parts first, while the sum that each addition cuts off is still small)
 #pragma unroll
-                for (int c = 0; c < D / CHUNK; ++c) {
-                    const uint32_t b = k_desc + after(stage, c / (SC / CHUNK)) * (STAGE >> 4) + c % (SC / CHUNK) * (CHUNK_BYTES >> 4);
+                for (int z = Z - 1; z >= 0; --z)
 #pragma unroll
-                    for (int z = 0; z < Z; ++z) {
+                    for (int c = 0; c < D / CHUNK; ++c) {
+                        const uint32_t b = k_desc + after(stage, c / (SC / CHUNK)) * (STAGE >> 4) + c % (SC / CHUNK) * (CHUNK_BYTES >> 4);
                         const uint32_t a = q_desc + ((KEYS ? 0 : i) * Z + z) * (QTILE >> 4) + c * (CHUNK_BYTES >> 4);
 #pragma unroll
-                        for (int e = 0; e < CHUNK / 16; ++e) mma_ss(d, a + e * 2, b + e * 2, id_s, c + e + z > 0);
+                        for (int e = 0; e < CHUNK / 16; ++e) mma_ss(d, a + e * 2, b + e * 2, id_s, z < Z - 1 || c + e > 0);
                     }
-                }
                 mma_commit(&bars.s_full[buf]);
             }
         };
@@ -210,10 +210,10 @@ struct Tiles {
                 for (int p = 0; p < PARTS; ++p) {
                     const uint32_t b = v_desc + after(stage, p) * (STAGE >> 4), d = tmem + 256 + i * D + p * SC;
 #pragma unroll
-                    for (int z = 0; z < Z; ++z)
+                    for (int z = Z - 1; z >= 0; --z)
 #pragma unroll
                         for (int e = e0; e < e1; ++e)
-                            mma_ts(d, tmem + buf * 128 + z * 64 + e * 8, b + e * (16 * 128 >> 4), id_o, add || e + z > e0);
+                            mma_ts(d, tmem + buf * 128 + z * 64 + e * 8, b + e * (16 * 128 >> 4), id_o, add || z < Z - 1 || e > e0);
                 }
             }
         };
