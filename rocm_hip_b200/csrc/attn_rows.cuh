@@ -8,6 +8,8 @@
 #ifndef B200_ATTN_ROWS_CUH
 #define B200_ATTN_ROWS_CUH
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace b200 {
