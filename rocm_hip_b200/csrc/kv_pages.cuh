@@ -227,6 +227,7 @@ k_kv_pages_resize(b200_kv_pages kv, const int* new_lens, int* slots, int n_slots
     const int s_first = cta + CTAS * (threadIdx.x >> 5), s_step = CTAS * (KVP_THREADS / 32);
     for (int s = s_first; s < kv.n_seqs; s += s_step) {
         const int to = new_lens[s], n = kvp_len(kv, s);
+        __syncwarp();   // every lane has read the length before lane 0 writes it
         if (to < 0 || to >= n) continue;
         int* row = kv.table + (long long)s * kv.max_pages;
         const int stay = kvp_pages(to, kv.page_shift), had = kvp_pages(n, kv.page_shift);
