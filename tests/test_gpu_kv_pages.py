@@ -309,14 +309,16 @@ def test_serving_run(ops):
     decode([2, 3], q[[2, 3]].contiguous(), 288)
 
 
-def test_many_sequences_cut_back_at_once(ops):
+@pytest.mark.parametrize("n_seqs", [150, 400])     # (one CTA, a cluster)
+def test_many_sequences_cut_back_at_once(ops, n_seqs):
     """A warp cuts back several sequences one after another, lanes giving back different numbers of pages each: every page
     that is no longer needed is free, none of them twice."""
     r = random.Random(3)
-    x = Both(ops, 400, 90, 20000, 1)
+    n_pages = n_seqs * 90
+    x = Both(ops, n_seqs, 90, n_pages, 1)
     for _ in range(6):
         x.resize([r.choice([0, 1, 63, 64, 65, 66, 130, 180]) if n == 0 else -1 for n in x.m.lens])
         assert x.m.info[0] == 0
         x.resize([r.randint(0, n) if r.random() < 0.9 else -1 for n in x.m.lens])
-    x.resize([0] * 400)
-    assert x.m.info[1] == 20000
+    x.resize([0] * n_seqs)
+    assert x.m.info[1] == n_pages
