@@ -118,8 +118,8 @@ cudaError_t launch_prompt(const T* q, const T* k, const T* v, T* out, const int*
         static std::atomic<unsigned long long> done;                                                                         \
         st = allow_smem(k_attn_prompt<D_, T, MODE_>, SMEM, done);                                                                  \
         if (st != cudaSuccess) return st;                                                                                    \
-        launch_pdl((k_attn_prompt<D_, T, MODE_>), (unsigned)grid, Ti::WARPS * 32, SMEM, stream, mq, mk, mv, q, k, v, out, seq_start, \
-                   n_seqs, (int)rows, n_q, n_q / n_kv, q_stride, k_stride, v_stride, scale * LOG2E, (int)n_slots);           \
+        launch_pdl((k_attn_prompt<D_, T, MODE_>), (unsigned)grid, PROMPT_WARPS<D_> * 32, SMEM, stream, mq, mk, mv, v, out, seq_start,  \
+                   n_seqs, (int)rows, n_q, n_q / n_kv, v_stride, scale * LOG2E, (int)n_slots);                               \
     } while (0)
 #define MODES(D_)                                                                                                            \
     do {                                                                                                                     \

@@ -77,7 +77,7 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                 if (lane < boxes)
                     for (int c = 0; c < SC / CHUNK; ++c)
                         tma_4d(dst + c * CHUNK_BYTES + lane * box * 128, map, p * SC + c * CHUNK, kh, row, page, bar);
-            });
+            }, bars.full);
         };
         int p0 = page_of(0), p1 = page_of(1), p2 = page_of(2);
         put(&mk, 0, p0);

@@ -30,10 +30,106 @@ struct PromptItem {
     int n[2];                   // key tiles per query tile; n[0] == 0: there is nothing more
 };
 struct PromptBars {
-    unsigned long long item_full[2], item_empty[2], q_empty[2], asked, ml_full, o_read;
+    unsigned long long item_full[2], item_empty[2], q_empty[2], asked, ml_full, o_read, raw[8], looked[4];
     uint4 answer;               // of the work distributor, 16 bytes
     PromptItem item[2];
+    unsigned odd[4][2][4];      // of four items in turn, of their up to two tiles looked at: the keys whose v was blanked
 };
+
+// Softmax warps, tensor cores, copies, schedule, and one that looks at V tiles
+template <int D>
+constexpr int PROMPT_WARPS = D == 256 ? 8 : 12;
+
+// A weight of 0 times a non-finite v is not 0 on the tensor cores, and a query tile's last key tile holds keys that some of its
+// rows do not see: later ones, the next sequence's, rows in no sequence. So from the first query tile's last key tile on
+// (one tile, or two where the query tiles are 256 rows of one head) the copies of V report to a warp of its own, which blanks
+// what is not finite and then hands the tile to the tensor cores; rows get back what they do see of that with plain
+// additions, an infinity or a NaN as it is. What a row does not see can then change no bit of its result, and what the
+// hand-over costs is one packed multiply-add per pair of values (v 0 + 0 is NaN for them), while the tile's scores are in the
+// softmax: 61 sequences of 64-wide heads 62.5 -> 66.9 us, one sequence of 2,427 rows 38.8 -> 37.9, 32,768 rows 2.78 -> 2.76 ms
+// against rows that were computed again, key after key, when they came out non-finite, which took the softmax warps out of
+// the CTA's pipeline for as long as a sequence has keys. (The tensor cores' warp asking for the look when it takes a tile:
+// two more waits in its loop cost 11 % of long prompts. By mma.sync in place of the multiply-adds: no faster.)
+
+// v 0 + acc for pairs: NaN from the first value on that is not finite
+template <typename T>
+__device__ __forceinline__ uint32_t mark_non_finite(uint32_t w, uint32_t acc) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(acc));
+    else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0u), "r"(acc));
+    return r;
+}
+
+// One warp: blanks what is not finite in BYTES of a V tile of 128 rows, [values / 64][128 rows][64 values], and sets the bits of
+// its rows
+template <typename T, int BYTES>
+__device__ __forceinline__ void blank_non_finite(unsigned char* part, unsigned* odd) {
+    constexpr uint32_t EXP = std::is_same<T, __nv_bfloat16>::value ? 0x7f80u : 0x7c00u;
+    constexpr int AT_ONCE = 8;
+    static_assert(BYTES % (AT_ONCE * 512) == 0, "whole rounds");
+    const int lane = threadIdx.x & 31;
+    uint32_t acc[4] = {0, 0, 0, 0};
+    for (int at = lane * 16; at < BYTES; at += AT_ONCE * 512) {
+        uint4 w[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) w[i] = *reinterpret_cast<const uint4*>(part + at + i * 512);
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            acc[0] = mark_non_finite<T>(w[i].x, acc[0]);
+            acc[1] = mark_non_finite<T>(w[i].y, acc[1]);
+            acc[2] = mark_non_finite<T>(w[i].z, acc[2]);
+            acc[3] = mark_non_finite<T>(w[i].w, acc[3]);
+        }
+    }
+    // (the sums are +-0 or NaN)
+    if (!__any_sync(0xffffffffu, (acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu)) return;
+    for (int at = lane * 16; at < BYTES; at += 512) {
+        uint4 w = *reinterpret_cast<const uint4*>(part + at);
+        const auto blank = [](uint32_t x) {
+            if ((x & EXP) == EXP) x &= 0xffff0000u;
+            if ((x >> 16 & EXP) == EXP) x &= 0x0000ffffu;
+            return x;
+        };
+        const uint4 b = make_uint4(blank(w.x), blank(w.y), blank(w.z), blank(w.w));
+        if (b.x != w.x || b.y != w.y || b.z != w.z || b.w != w.w) {
+            *reinterpret_cast<uint4*>(part + at) = b;
+            const int row = at / 128 % TILE_ROWS;
+            atomicOr(odd + row / 32, 1u << row % 32);
+        }
+    }
+    fence_async_smem();          // the tensor cores read through the other proxy
+}
+
+// What blank_non_finite took from the rows of a warp that see it, added to them: `word` of lanes 0 .. 7 are the bits of the
+// blanked keys, v0 the first of these keys, `from` that key's distance to the warp's first row, `rows` how many rows it has,
+// out the first one. Lanes in `mine` look after their columns.
+template <int D, typename T>
+__device__ void give_non_finite(unsigned word, const T* v0, long long v_stride, int from, int rows, T* out, long long out_stride, unsigned mine) {
+    constexpr int N = D / 32;
+    const int lane = threadIdx.x & 31, c = lane * N;
+    float sum[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+    for (int r = 0, k = 0; r < rows; ++r) {
+        for (; k <= from + r; ++k) {            // the keys up to the row's own
+            if (!(__shfl_sync(0xffffffffu, word, k >> 5) >> (k & 31) & 1)) continue;
+            float x[N];
+            load_vals(v0 + k * v_stride + c, x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += fabsf(x[i]) < INFINITY ? 0.0f : x[i];
+        }
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i) any |= sum[i] != 0.0f;
+        if (any && (mine >> lane & 1)) {
+            float y[N];
+            load_vals(out + r * out_stride + c, y);
+#pragma unroll
+            for (int i = 0; i < N; ++i) y[i] += sum[i];
+            store_vals(out + r * out_stride + c, y);
+        }
+    }
+}
 
 // The next block of the grid that has not begun, taken over by this CTA (the hardware's work distributor hands blocks to CTAs
 // that ask as it hands them to SMs that are free): asks, and later reads the answer. One thread.
@@ -60,10 +156,9 @@ __device__ __forceinline__ int block_answer(PromptBars& pb) {   // the block's i
 // soon as the query tile's memory is free and filled again. (One CTA per block: 61 sequences of 200 rows, 16 heads of 64, took 98 us, most of
 // it the way from a CTA's start to its first product and from its last to its end.)
 template <int D, typename T, int MODE>
-__global__ void __launch_bounds__(PromptTiles<D, T>::WARPS * 32, 1)
+__global__ void __launch_bounds__(PROMPT_WARPS<D> * 32, 1)
 k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
-              const T* q, const T* k, const T* v, T* out, const int* seq_start, int n_seqs, int rows, int n_q, int G,
-              long long q_stride, long long k_stride, long long v_stride, float scale2, int n_slots) {
+              const T* v, T* out, const int* seq_start, int n_seqs, int rows, int n_q, int G, long long v_stride, float scale2, int n_slots) {
     using Ti = PromptTiles<D, T>;
     constexpr int NQ = D == 256 ? 1 : 2, SC = D < 128 ? D : 128;
     constexpr int ROWS = NQ == 2 && MODE == BY_ROWS ? 2 * TILE_ROWS : TILE_ROWS;                       // of a block
@@ -81,12 +176,14 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         tma_prefetch(&mv);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&pb.item_full[i], 1);
-            mbar_init(&pb.item_empty[i], NQ * 4 + 2);
+            mbar_init(&pb.item_empty[i], NQ * 4 + 3);
             mbar_init(&pb.q_empty[i], PROMPT_OUT<D> ? 1 : MODE == BY_KEYS ? 8 : 4);
         }
         mbar_init(&pb.asked, 1);
         mbar_init(&pb.ml_full, 8);
         mbar_init(&pb.o_read, 8);
+        for (int i = 0; i < Ti::STAGES; ++i) mbar_init(&pb.raw[i], 1);
+        for (int i = 0; i < 4; ++i) mbar_init(&pb.looked[i], 1);
         mbar_fence_init();
     }
     Ti::setup(bars, 1);
@@ -172,10 +269,10 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         unsigned items[2] = {0, 0};
         while (next_item(&it)) {
             const int kh = it.h / G, n_all = max(it.n[0], it.n[1]);
-            const auto put = [&](const CUtensorMap* map, int j) {
+            const auto put = [&](const CUtensorMap* map, int j, bool look = false) {
                 r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
                     if (lane < SC / CHUNK) tma_3d(dst + lane * CHUNK_BYTES, map, p * SC + lane * CHUNK, kh, it.first + j * TILE_ROWS, bar);
-                });
+                }, look ? pb.raw : bars.full);
             };
             put(&mk, 0);
 #pragma unroll
@@ -191,7 +288,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             if (MODE == BY_KEYS && n_all > 1) put(&mk, 1);
             for (int j = 0; j < n_all; ++j) {
                 if (MODE != BY_KEYS && j + 1 < n_all) put(&mk, j + 1);
-                put(&mv, j);
+                put(&mv, j, j + 1 >= it.n[0]);
                 if (MODE == BY_KEYS && j + 2 < n_all) put(&mk, j + 2);
             }
         }
@@ -201,6 +298,35 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
         PromptItem it;
         while (next_item(&it))
             if (!Ti::template products<MODE == BY_KEYS>(bars, smem, ring, it.n[0], it.n[1], f, PROMPT_OUT<D> ? pb.q_empty : nullptr)) break;
+    } else if (warp == NQ * 4 + 3) {
+        Ti::few_registers();
+        // ---- looks: V tiles in which a row may have unseen keys, where the ring has them (K 0, K 1, V 0, K 2, V 1, .., V n - 1)
+        PromptItem it;
+        unsigned parity = 0;      // bit s: of stage s's next copy that reports here
+        int base = 0;             // the stage of the item's K 0
+        bool ok = true;
+        while (ok && next_item(&it)) {
+            const int n_all = max(it.n[0], it.n[1]), slot = taken - 1 & 3;
+            if (lane < 8) pb.odd[slot][lane >> 2][lane & 3] = 0;
+            __syncwarp();
+#pragma unroll 1
+            for (int j = it.n[0] - 1; ok && j < n_all; ++j) {
+                const int at = (base + (j + 1 < n_all ? 2 * j + 2 : 2 * n_all - 1) % Ti::STAGES * Ti::PARTS) % Ti::STAGES;
+#pragma unroll 1
+                for (int p = 0; ok && p < Ti::PARTS; ++p) {
+                    const int st = at + p < Ti::STAGES ? at + p : at + p - Ti::STAGES;
+                    ok = warp_wait_long(&pb.raw[st], parity >> st & 1, &bars.dead);
+                    parity ^= 1u << st;
+                    if (ok) blank_non_finite<T, Ti::STAGE>(ring + st * Ti::STAGE, pb.odd[slot][j - (it.n[0] - 1)]);
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (j + 1 == n_all && p + 1 == Ti::PARTS) mbar_arrive(&pb.looked[slot]);
+                        mbar_arrive(&bars.full[st]);
+                    }
+                }
+            }
+            base = (base + 2 * n_all % Ti::STAGES * Ti::PARTS) % Ti::STAGES;
+        }
     } else if (warp < NQ * 4) {
         Ti::many_registers();
         // ---- softmax: thread = row
@@ -224,7 +350,9 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                             if (e > seen) x[e] = 0xff800000u;
                 });
             }
-            if (!ok) break;
+            // (behind this item's last weights, where there is nothing else to do until their products are done)
+            if (!ok || !warp_wait(&pb.looked[taken - 1 & 3], taken - 1 >> 2 & 1, &bars.dead)) break;
+            const unsigned odd = lane < 8 ? pb.odd[taken - 1 & 3][lane >> 2][lane & 3] : 0;
             // the weights of the two halves' O, 1 / l included
             float w0 = 1.0f, w1 = 0.0f;
             if constexpr (MODE == BY_KEYS) {
@@ -256,7 +384,6 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             const uint32_t o_addr = bars.tmem + 256 + (MODE == BY_KEYS ? 0 : i * D) + at0 + ((uint32_t)(threadIdx.x & 96) << 16);
             unsigned char* mine = BUF ? ring + Ti::RING + warp * 2048
                                       : smem + ((MODE == BY_KEYS ? 0 : i * TILE_ROWS) + (warp & 3) * 32) * (D * 2) + at0 * 2;
-            bool bad = false;
             for (int c0 = 0; c0 < COLS; c0 += CW) {
                 for (int c = 0; c < CW; c += 32) {
                     uint32_t o[32], o1[MODE == BY_KEYS ? 32 : 1];
@@ -275,7 +402,6 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                                 const float both = fmaf(__uint_as_float(o1[e + t]), w1, y[t]);
                                 y[t] = tiles > 1 ? both : y[t];
                             }
-                            bad |= !(fabsf(y[t]) < INFINITY);
                         }
                         // (units of 16 bytes, stirred so that neither eight lanes' rows nor eight units share a bank)
                         const int u = (c + e) / 8, at = BUF ? u ^ (lane >> 1 & 3) : u ^ (lane & 7);
@@ -302,35 +428,17 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&pb.o_read);
             }
-            // A weight of 0 times a non-finite v is not 0 on the tensor cores. Rows that came out non-finite are computed again from
-            // the keys they see, where a key of the last tile that they do not see has such a v.
-            unsigned again = __ballot_sync(0xffffffffu, bad && row < end);
-            __syncwarp();
-            if (again) {
-                const int d0 = first + (tiles - 1) * TILE_ROWS;      // the last tile's first key
-                unsigned non_finite[4];
-                find_non_finite<D>(v + d0 * v_stride + h / G * D, v_stride, min(TILE_ROWS, rows - d0), non_finite);
-                while (again) {
-                    const int t = t0 + (warp & 3) * 32 + __ffs(again) - 1, seen = t - d0;
-                    again &= again - 1;
-                    bool unseen = false;
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int k = seen + 1 - 32 * w;             // first bit of this word that the row does not see
-                        unseen |= (k <= 0 ? non_finite[w] : k < 32 ? non_finite[w] >> k : 0) != 0;
-                    }
-                    if (unseen)
-                        attn_row_again<D, T>(q + t * q_stride + h * D, k + first * k_stride + h / G * D, v + first * v_stride + h / G * D,
-                                             k_stride, v_stride, t - first + 1, scale2, out + ((long long)t * n_q + h) * D,
-                                             MODE != BY_KEYS ? 0xffffffffu : i ? 0xffff0000u : 0xffffu);
-                }
+            // What was blanked in the tiles that were looked at goes to the rows that see it
+            if (__any_sync(0xffffffffu, odd != 0)) {
+                const int k0 = first + (it.n[0] - 1) * TILE_ROWS, t = t0 + (warp & 3) * 32;
+                give_non_finite<D, T>(odd, v + k0 * v_stride + h / G * D, v_stride, t - k0, min(32, end - t),
+                                      out + ((long long)t * n_q + h) * D, (long long)n_q * D,
+                                      MODE != BY_KEYS ? 0xffffffffu : i ? 0xffff0000u : 0xffffu);
             }
             if constexpr (MODE == BY_KEYS) {
                 if (!warp_wait(&pb.o_read, (f.items[0] - 1) & 1, &bars.dead)) break;
             }
         }
-    } else {
-        Ti::few_registers();
     }
     Ti::teardown(bars);
 }

@@ -78,13 +78,13 @@ __device__ __forceinline__ bool warp_wait_long(unsigned long long* bar, unsigned
 // SC: columns of a ring stage (a K or V tile is D / SC stages of 128 rows), ST: stages
 template <int D, int NQ, int SC, int ST, bool SPLIT, typename T>
 struct Tiles {
-    static constexpr int STAGE = TILE_ROWS * SC * 2;
+    static constexpr int STAGE = TILE_ROWS * SC * 2, STAGES = ST;
     static constexpr int PARTS = D / SC;
     static constexpr int QTILE = TILE_ROWS * D * 2;                        // one query tile, one half of a split one
     static constexpr int Q_BYTES = NQ * QTILE * (SPLIT ? 2 : 1);           // [NQ][hi, lo][D / 64][128 rows][64 values]
     static constexpr int RING = ST * STAGE;
     static constexpr int SMEM = 1024 + Q_BYTES + RING;
-    static constexpr int WARPS = NQ == 2 ? 12 : 7;                         // softmax, tensor cores, copies, schedule (and an idle one)
+    static constexpr int WARPS = NQ == 2 ? 12 : 7;                         // softmax, tensor cores, copies, two more (prompts: eight of one query tile)
     // NQ = 2: the products of a tile's first half of the keys begin while the second half is still in the softmax (8,192 rows,
     // 32 heads of 128: 1,246 -> 1,295 TFLOP/s). With one query tile the next S fills that time (heads of 256: 1,286 without,
     // 1,261 with).
@@ -135,21 +135,22 @@ struct Tiles {
     }
 
     // The ring as the copying warp sees it: `load(smem, part, bar)` issues the copies of one stage, each lane its share of
-    // them. One lane waits, so that all of them go on or stop together.
+    // them. One lane waits, so that all of them go on or stop together. full: what the copies report to, bars.full or, for
+    // tiles that somebody looks at before the tensor cores may have them (and then arrives on bars.full), barriers of that one's.
     struct Ring {
         TileBars& bars;
         unsigned char* ring;
         int st = 0, ph = 0;
         template <typename F>
-        __device__ __forceinline__ void put(F load) {
+        __device__ __forceinline__ void put(F load, unsigned long long* full) {
             for (int p = 0; p < PARTS; ++p) {
                 int ok = 0;
                 if ((threadIdx.x & 31) == 0) {
                     ok = wait_or_die(&bars.empty[st], ph ^ 1, &bars.dead);
-                    if (ok) mbar_expect(&bars.full[st], STAGE);
+                    if (ok) mbar_expect(&full[st], STAGE);
                 }
                 if (!__shfl_sync(0xffffffffu, ok, 0)) return;
-                load(ring + st * STAGE, p, &bars.full[st]);
+                load(ring + st * STAGE, p, &full[st]);
                 if (++st == ST) { st = 0; ph ^= 1; }
             }
         }

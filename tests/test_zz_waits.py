@@ -1,0 +1,9 @@
+"""Collected behind every other GPU test: none of the attention kernels' waits has run out in any of them."""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_no_block_gave_up(ops):
+    from rocm_hip_b200 import _lib
+    assert _lib.load().b200_attn_gave_up() == 0
