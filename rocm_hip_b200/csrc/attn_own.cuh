@@ -184,7 +184,6 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
 
     unsigned char* ring = smem + warp * ST * Sh::STAGE;
     unsigned phases = 0;                    // bit s: the parity stage s completes next
-    bool alive = true;
     const int wu = warp % pl.wh, rg = warp / pl.wh;
     const int g8 = lane >> 2, t4 = lane & 3;
     for (; t0 < t_end && b < B; ++b, in_seq = 0) {
@@ -302,7 +301,7 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                         unsigned char* Kt = ring + s * Sh::STAGE;
                         unsigned char* Vt = Kt + 16 * D * 2;
                         if constexpr (BOX) {
-                            if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&full[warp][s], phases >> s & 1));
+                            if (!__all_sync(0xffffffffu, mbar_wait(&full[warp][s], phases >> s & 1))) goto gave_up;
                             phases ^= 1u << s;
                             if (seen[s] != 0xffffu) {   // a weight of 0 needs a finite v: what lies behind the sequence is blanked
                                 for (int e = lane; e < 16 * UNITS; e += 32)
@@ -405,7 +404,10 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
         }
     }
     if (!BOX) cp_async_wait_all();
-    if (!alive && lane == 0) atomicAdd(&attn_gave_up, 1);
+    return;
+gave_up:                                    // no copy may still be under way when the CTA ends and its memory becomes another's
+    for (int i = 0; i < ST; ++i) (void)mbar_wait(&full[warp][i], phases >> i & 1);
+    if (lane == 0) atomicAdd(&attn_gave_up, 1);
 }
 
 // The pieces the prefix kernel leaves: [split][key head][row b G + g]

@@ -77,7 +77,7 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
                 if (lane < boxes)
                     for (int c = 0; c < SC / CHUNK; ++c)
                         tma_4d(dst + c * CHUNK_BYTES + lane * box * 128, map, p * SC + c * CHUNK, kh, row, page, bar);
-            }, bars.full);
+            });
         };
         int p0 = page_of(0), p1 = page_of(1), p2 = page_of(2);
         put(&mk, 0, p0);
@@ -89,10 +89,12 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             p1 = p2;
             p2 = p3;
         }
+        Ti::copies_done(bars, r, nullptr, {0, 0});
     } else if (warp == NQ * 4) {
         Ti::few_registers();
         TileFlow f;
         Ti::products(bars, smem, ring, n[0], n[1], f);
+        Ti::products_done(bars);
     } else if (warp < NQ * 4) {
         Ti::many_registers();
         const int i = warp >> 2, mine = r0 + warp * 32;     // this warp's 32 query rows

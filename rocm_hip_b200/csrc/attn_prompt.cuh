@@ -261,6 +261,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             fence_async_smem();          // the answer has been read before the next one may arrive
             __syncwarp();
         }
+        if (block >= 0) (void)mbar_wait(&pb.asked, asked & 1);      // (given up with a question open)
     } else if (warp == NQ * 4 + 1) {
         Ti::few_registers();
         // ---- copies: K and V tiles in the order the tensor cores take them, and Q as soon as its place is free
@@ -272,7 +273,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
             const auto put = [&](const CUtensorMap* map, int j, bool look = false) {
                 r.put([&](unsigned char* dst, int p, unsigned long long* bar) {
                     if (lane < SC / CHUNK) tma_3d(dst + lane * CHUNK_BYTES, map, p * SC + lane * CHUNK, kh, it.first + j * TILE_ROWS, bar);
-                }, look ? pb.raw : bars.full);
+                }, look ? pb.raw : nullptr);
             };
             put(&mk, 0);
 #pragma unroll
@@ -292,12 +293,14 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                 if (MODE == BY_KEYS && j + 2 < n_all) put(&mk, j + 2);
             }
         }
+        Ti::copies_done(bars, r, pb.raw, items);
     } else if (warp == NQ * 4) {
         Ti::few_registers();
         TileFlow f;
         PromptItem it;
         while (next_item(&it))
             if (!Ti::template products<MODE == BY_KEYS>(bars, smem, ring, it.n[0], it.n[1], f, PROMPT_OUT<D> ? pb.q_empty : nullptr)) break;
+        Ti::products_done(bars);
     } else if (warp == NQ * 4 + 3) {
         Ti::few_registers();
         // ---- looks: V tiles in which a row may have unseen keys, where the ring has them (K 0, K 1, V 0, K 2, V 1, .., V n - 1)

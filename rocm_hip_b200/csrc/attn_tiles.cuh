@@ -21,7 +21,7 @@ namespace b200 {
 __device__ int attn_gave_up;
 
 struct TileBars {
-    unsigned long long q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_part, full[8], empty[8];
+    unsigned long long q_full[2], s_full[2], p_half[2], p_full[2], o_full[2], o_part, quiet, full[8], empty[8];
     uint32_t tmem;
     int dead;
 };
@@ -108,6 +108,7 @@ struct Tiles {
             tmem_alloc(&bars.tmem, 512);
             if ((threadIdx.x & 31) == 0) {
                 mbar_init(&bars.o_part, 1);
+                mbar_init(&bars.quiet, 1);
                 for (int i = 0; i < 2; ++i) {
                     mbar_init(&bars.q_full[i], q_arrivals);
                     mbar_init(&bars.s_full[i], 1);
@@ -135,14 +136,16 @@ struct Tiles {
     }
 
     // The ring as the copying warp sees it: `load(smem, part, bar)` issues the copies of one stage, each lane its share of
-    // them. One lane waits, so that all of them go on or stop together. full: what the copies report to, bars.full or, for
-    // tiles that somebody looks at before the tensor cores may have them (and then arrives on bars.full), barriers of that one's.
+    // them. One lane waits, so that all of them go on or stop together. The copies report to bars.full or, for tiles that
+    // somebody looks at before the tensor cores may have them (and then arrives on bars.full), to `others`.
     struct Ring {
         TileBars& bars;
         unsigned char* ring;
         int st = 0, ph = 0;
+        unsigned other = 0, turn = 0;     // bit s: stage s's last copies reported to the other barriers; parity of the next such
         template <typename F>
-        __device__ __forceinline__ void put(F load, unsigned long long* full) {
+        __device__ __forceinline__ void put(F load, unsigned long long* others = nullptr) {
+            unsigned long long* full = others ? others : bars.full;
             for (int p = 0; p < PARTS; ++p) {
                 int ok = 0;
                 if ((threadIdx.x & 31) == 0) {
@@ -151,10 +154,28 @@ struct Tiles {
                 }
                 if (!__shfl_sync(0xffffffffu, ok, 0)) return;
                 load(ring + st * STAGE, p, &full[st]);
+                const unsigned bit = 1u << st;
+                if (others) { other |= bit; turn ^= bit; } else other &= ~bit;
                 if (++st == ST) { st = 0; ph ^= 1; }
             }
         }
     };
+
+    // The end of a role, also of one that gave up: nothing that it started is still under way when the CTA ends and its memory,
+    // shared or tensor, becomes another's. Where all went well both are there already or about to be.
+    static __device__ __forceinline__ void copies_done(TileBars& bars, const Ring& r, unsigned long long* others, const unsigned (&queries)[2]) {
+#pragma unroll 1
+        for (int i = 0; i < ST; ++i) {
+            if (r.other >> i & 1) (void)mbar_wait(&others[i], (r.turn >> i & 1) ^ 1);
+            else (void)mbar_wait(&bars.full[i], i < r.st ? r.ph : r.ph ^ 1);     // (a stage never used: the phase before the first)
+        }
+        for (int i = 0; i < 2; ++i)
+            if (queries[i]) (void)mbar_wait(&bars.q_full[i], (queries[i] - 1) & 1);
+    }
+    static __device__ __forceinline__ void products_done(TileBars& bars) {
+        if (elect_one()) mma_commit(&bars.quiet);
+        (void)mbar_wait(&bars.quiet, 0);
+    }
 
     static __device__ __forceinline__ int buffer(unsigned steps, int i) { return NQ == 1 ? steps & 1 : i; }
     static __device__ __forceinline__ unsigned parity(unsigned steps) { return NQ == 1 ? steps >> 1 & 1 : steps & 1; }
