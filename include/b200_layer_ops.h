@@ -538,9 +538,10 @@ int b200_attn_gave_up(void);
  * pages[b][t >> kv_shift] (pages: [B][max_pages] ints), and row r of page p is at K + p * kv_bstride + r * kv_stride
  * values, V likewise: the block-major cache that gpu_kv_store_f16 writes, with positions = p * 2^kv_shift + r. Ids outside
  * [0, n_pages) are rows that are not seen. lens[b] <= 0: out[b] is zero.
- * prefix_len > 0: every sequence with lens[b] >= prefix_len begins with the same prefix_len rows IN THE SAME PAGES (as
- * gpu_kv_pages_fork leaves them), which are then read once for the whole batch; a multiple of 2^kv_shift. Sequences with
- * fewer rows (idle slots) use their own pages only. Memory behind lens[b] may hold anything; a page of up to 4096 rows is
+ * prefix_len > 0, a multiple of 2^kv_shift: the first prefix_len rows of the batch's first sequence with lens[b] >= prefix_len
+ * are read once for all sequences of at least that length whose page lists begin with the SAME pages (as gpu_kv_pages_fork
+ * leaves them). The call compares the lists: sequences with other pages in their place, or fewer rows, read their own.
+ * Memory behind lens[b] may hold anything; a page of up to 4096 rows is
  * readable to its end, of larger ones (a contiguous cache: kv_shift 30, one page per sequence) nothing behind lens[b] is
  * touched.
  * fp32 rows come out to a few 1e-6 of the result's norm (two fp16 values a query value and weight). kv_stride and

@@ -150,7 +150,7 @@ bool page_map(CUtensorMap* m, const __half* p, int D, int heads, const PagedKv& 
 struct DecodePlan {
     int grid_own, nq, row_tiles, splits;     // splits 0: nothing is shared
     long long px_rows;
-    size_t first, own_ml, own_o, px_ml, px_o, bytes;
+    size_t first, shares, own_ml, own_o, px_ml, px_o, bytes;
 
     DecodePlan(int n_q, int n_kv, int D, int B, int prefix, bool f32) {
         const int warps = D == 256 ? OwnShape<256>::WARPS : OwnShape<128>::WARPS, sms = sm_count();
@@ -187,6 +187,7 @@ struct DecodePlan {
         };
         bytes = 256;
         first = put(((size_t)B + 1) * 4);
+        shares = put((size_t)B * 4);
         own_ml = put(pieces * 8);
         own_o = put(pieces * D * 4);
         const size_t px = (size_t)splits * n_kv * px_rows;
@@ -200,8 +201,6 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
                             const DecodePlan& pl, cudaStream_t stream) {
     constexpr bool SPLIT = sizeof(T) == 4;
     const OwnPlan own(n_q, n_kv, OwnShape<D>::WARPS);
-    const OwnScratch sc{reinterpret_cast<int*>(scratch), reinterpret_cast<int*>(scratch + pl.first),
-                        reinterpret_cast<float*>(scratch + pl.own_ml), reinterpret_cast<float*>(scratch + pl.own_o)};
     // The copy engine takes the cache apart where pages are whole swizzle atoms (8 rows) and a tensor map can describe it;
     // else a prefix is read like every sequence's own rows, and those by the threads. It fetches 16 rows at a time, so a
     // sequence's last fetch may reach behind its rows, to the page's end at most: pages of more than 4,096 rows (a contiguous
@@ -214,7 +213,14 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
     const PrefixScratch px{shared ? pl.splits : 0, pl.px_rows, reinterpret_cast<float*>(scratch + pl.px_ml),
                            reinterpret_cast<float*>(scratch + pl.px_o)};
     const int behind = shared ? prefix : 0;
+    const OwnScratch sc{reinterpret_cast<int*>(scratch), reinterpret_cast<int*>(scratch + pl.first),
+                        shared ? reinterpret_cast<int*>(scratch + pl.shares) : nullptr, reinterpret_cast<float*>(scratch + pl.own_ml),
+                        reinterpret_cast<float*>(scratch + pl.own_o)};
     cudaError_t st;
+    if (shared) {
+        launch_pdl(k_attn_shares, (unsigned)B, SHARES_THREADS, 0, stream, kv, sc.shares, B, prefix);
+        if ((st = launched()) != cudaSuccess) return st;
+    }
 #define OWN(BOX_)                                                                                                            \
     do {                                                                                                                     \
         static std::atomic<unsigned long long> done;                                                                         \
@@ -242,8 +248,7 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
 #undef PREFIX
         if ((st = launched()) != cudaSuccess) return st;
     }
-    launch_pdl((k_attn_join<D, T>), (unsigned)(((long long)B * n_q + 3) / 4), 128, 0, stream, kv, sc, own, px, out, n_q, n_kv,
-               B, behind);
+    launch_pdl((k_attn_join<D, T>), (unsigned)(((long long)B * n_q + 3) / 4), 128, 0, stream, sc, own, px, out, n_q, n_kv, B);
     return launched();
 }
 

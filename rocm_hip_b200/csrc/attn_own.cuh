@@ -56,6 +56,7 @@ struct OwnPlan {
 struct OwnScratch {
     int* head;        // [0] tiles per CTA
     int* first;       // [B + 1] tiles before sequence b (of one group)
+    int* shares;      // [B] whether sequence b begins with the batch's prefix (k_attn_shares); null: nothing is shared
     float* ml;        // [slot][warp][hg][2]
     float* o;         // [slot][warp][hg][D]
 };
@@ -90,11 +91,10 @@ __device__ __forceinline__ int q_exponent(float top) {
     const int x = (__float_as_int(top) >> 23) & 255;
     return top > 0.0f && x < 255 ? 9 + 127 - (x ? x : 1) : 0;
 }
-// Rows of its own that sequence b has, and where they begin: behind the shared prefix if it has it whole
-__device__ __forceinline__ int own_rows(const PagedKv& kv, int b, int prefix, int* start) {
-    const int n = kv.len(b);
-    *start = n >= prefix ? prefix : 0;
-    return n - *start;
+// Rows of its own that sequence b has, and where they begin: behind the shared prefix if it has that
+__device__ __forceinline__ int own_rows(const PagedKv& kv, const OwnScratch& sc, int b, int prefix, int* start) {
+    *start = sc.shares && sc.shares[b] ? prefix : 0;
+    return kv.len(b) - *start;
 }
 
 // QT: type of the queries (fp32: two fp16 values per query value and weight). BOX: tiles come by the copy engine, in boxes
@@ -125,7 +125,7 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
     // ---- the shares: every CTA sums the tiles of all sequences, then finds where its own share begins
     const auto tiles_of = [&](int b) {
         int s;
-        return b < B ? (own_rows(kv, b, prefix, &s) + tile - 1) / tile : 0;
+        return b < B ? (own_rows(kv, sc, b, prefix, &s) + tile - 1) / tile : 0;
     };
     const auto cta_scan = [&](int v, int* total) {
         int x = v;
@@ -188,7 +188,7 @@ k_attn_own(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
     const int g8 = lane >> 2, t4 = lane & 3;
     for (; t0 < t_end && b < B; ++b, in_seq = 0) {
         int start;
-        const int own = own_rows(kv, b, prefix, &start), n_tiles = (own + tile - 1) / tile;
+        const int own = own_rows(kv, sc, b, prefix, &start), n_tiles = (own + tile - 1) / tile;
         while (in_seq < n_tiles * pl.groups && t0 < t_end) {
             // ---- one piece: tiles [k0, k1) of group `grp` of sequence b
             const int grp = in_seq / n_tiles, k0 = in_seq - grp * n_tiles;
@@ -422,18 +422,17 @@ struct PrefixScratch {
 // cover; a row without pieces, or with none that saw a key, is zero. A warp per row.
 template <int D, typename QT>
 __global__ void __launch_bounds__(128)
-k_attn_join(PagedKv kv, OwnScratch sc, OwnPlan pl, PrefixScratch px, QT* out, int n_q, int n_kv, int B, int prefix) {
+k_attn_join(OwnScratch sc, OwnPlan pl, PrefixScratch px, QT* out, int n_q, int n_kv, int B) {
     pdl_entry();
     constexpr int N = D / 32, W = OwnShape<D>::WARPS;
     const int row = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;     // (B n_q <= 2^28)
     if (row >= B * n_q) return;
     const int b = row / n_q, h = row - b * n_q, G = n_q / n_kv, kh = h / G, g = h - kh * G;
     const int u = kh * pl.gt + g / 8, grp = u / pl.wh, wu = u - grp * pl.wh;
-    // (volatile: all four are under way before the first is needed; left to the compiler, two of them waited for the others)
+    // (volatile: all of them are under way before the first is needed; left to the compiler, two of them waited for the others)
     const int before = *(const volatile int*)(sc.first + b), n_tiles = *(const volatile int*)(sc.first + b + 1) - before;
     const long long per = *(const volatile long long*)sc.head;
-    const int len = *(const volatile int*)(kv.lens + b);
-    const int n_px = (long long)len >= prefix && ((long long)kv.max_pages << kv.kv_shift) >= prefix ? px.splits : 0;
+    const int n_px = px.splits && *(const volatile int*)(sc.shares + b) ? px.splits : 0;
     const long long t0 = (long long)before * pl.groups + (long long)grp * n_tiles, t1 = t0 + n_tiles - 1;
     int c0 = 0, n_own = 0;
     if (n_tiles > 0) {

@@ -1,0 +1,85 @@
+"""Single-token attention behind a shared prefix: which sequences share it is read from their page lists, not taken from their
+lengths. Against 64 bits with the bounds of test_gpu_attention.py."""
+import pytest
+import torch
+
+from test_gpu_attention import BF, F32, decode, decode_check, paged
+
+pytestmark = pytest.mark.gpu
+
+
+def queries(B, n_q, D, dt, seed=9):
+    return torch.randn(B, n_q * D, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda").to(dt)
+
+
+def own_prefix(pool, table, n_pages, spare, b, first, last, page, kv, seed):
+    """Sequence b gets pages of its own, with other rows, for its list's entries [first, last)."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    for i in range(first, last):
+        p = spare.pop()
+        pool[p, :, :, :kv] = torch.randn(2, page, kv, generator=g, device="cuda").to(pool.dtype)
+        table[b, i] = p
+
+
+# (which sequences have pages of their own, which entries of the prefix): the last page only, the first only, all; the first
+# sequence of the batch; all but one; all
+OTHERS = [((2,), "last"), ((2,), "first"), ((1, 4), "all"), ((0,), "last"), ((0, 1, 2, 3), "all"), ((0, 1, 2, 3, 4, 5), "first")]
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page,prefix", [(16, 512), (8, 256), (256, 768), (64, 2048)])
+@pytest.mark.parametrize("others,where", OTHERS)
+def test_sequences_with_pages_of_their_own(ops, others, where, page, prefix, D, dt):
+    n_q, n_kv, n = 6, 2, prefix // page
+    lens = [prefix, prefix + 70, prefix + 300, prefix + 1, prefix + 129, prefix + 16, prefix - 1, 0]
+    pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 31, spare=n * 6 + 3)
+    used = set(table.flatten().tolist())
+    spare = [p for p in range(n_pages) if p not in used]
+    for b in others:
+        own_prefix(pool, table, n_pages, spare, b, n - 1 if where == "last" else 0, 1 if where == "first" else n, page, n_kv * D, b)
+    q = queries(len(lens), n_q, D, dt)
+    out = decode(ops, q, pool, table, L, stride, n_pages, max_pages, page, prefix, n_q, n_kv, D, D ** -0.5)
+    decode_check(out, q, pool, table, L, page, n_q, n_kv, D, D ** -0.5)
+
+
+@pytest.mark.parametrize("B,n_q,n_kv", [(300, 4, 1), (70, 10, 2)])
+def test_a_mixed_batch(ops, B, n_q, n_kv):
+    """Two prompts' samples in one batch, in turn: those of the first share, the others read their own."""
+    D, page, prefix = 128, 16, 320
+    lens = [prefix + (7 * i) % 90 for i in range(B)]
+    pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 32, spare=30)
+    used = set(table.flatten().tolist())
+    spare = [p for p in range(n_pages) if p not in used]
+    own_prefix(pool, table, n_pages, spare, 1, 0, prefix // page, page, n_kv * D, 5)
+    table[3::2, :prefix // page] = table[1, :prefix // page].clone()
+    for dt in (F32, BF):
+        q = queries(B, n_q, D, dt)
+        out = decode(ops, q, pool, table, L, stride, n_pages, max_pages, page, prefix, n_q, n_kv, D, 0.1)
+        decode_check(out, q, pool, table, L, page, n_q, n_kv, D, 0.1)
+
+
+def test_captured_call_follows_the_lists(ops):
+    """A captured call, replayed while a sequence leaves the prefix and joins it again."""
+    D, page, prefix, n_q, n_kv = 128, 32, 512, 8, 2
+    lens = [prefix + 10 * i for i in range(5)]
+    pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 33, spare=40)
+    used = set(table.flatten().tolist())
+    spare = [p for p in range(n_pages) if p not in used]
+    other = table.clone()
+    own_prefix(pool, other, n_pages, spare, 3, 0, prefix // page, page, n_kv * D, 6)
+    shared = table.clone()
+    q, out = queries(5, n_q, D, F32), torch.empty(5, n_q * D, device="cuda")
+    scratch = torch.empty(ops.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, 5, prefix), dtype=torch.uint8, device="cuda")
+    call = lambda: ops.gpu_attn_decode(q, pool, pool[0, 1], stride, 5, 2 * page * stride, n_pages, table, max_pages, L, prefix, out, n_q,  # noqa: E731
+                                       n_kv, D, 5, 0.1, scratch)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for lists in (shared, other, shared, other):
+        table.copy_(lists)
+        scratch.fill_(0xff)
+        graph.replay()
+        decode_check(out, q, pool, table, L, page, n_q, n_kv, D, 0.1)
