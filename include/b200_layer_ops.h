@@ -547,7 +547,8 @@ int b200_attn_gave_up(void);
  * fp32 rows come out to a few 1e-6 of the result's norm (two fp16 values a query value and weight). kv_stride and
  * kv_bstride are multiples of 8, pointers 16-byte aligned, out is not q.
  * scratch: device memory of gpu_attn_decode_scratch_bytes(...) bytes, any contents, in use until the call has run; calls
- * that may overlap need scratch of their own. */
+ * that may overlap need scratch of their own. The bytes grow with B and prefix_len: what the largest batch behind the longest
+ * prefix needs serves every smaller call with the same heads, of either row type. */
 size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len);
 cudaError_t gpu_attn_decode(const float* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,
                             int n_pages, const int* pages, int max_pages, const int* lens, int prefix_len, float* out, int n_q,

@@ -146,7 +146,9 @@ bool page_map(CUtensorMap* m, const __half* p, int D, int heads, const PagedKv& 
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// What a decode call launches and where its pieces lie in scratch: a function of the sizes the host knows
+// What a decode call launches and where its pieces lie in scratch: a function of the sizes the host knows. `bytes` covers what
+// a call of either row type uses and grows with B and the prefix, so that the scratch of the largest call serves all smaller
+// ones.
 struct DecodePlan {
     int grid_own, nq, row_tiles, splits;     // splits 0: nothing is shared
     long long px_rows;
@@ -161,6 +163,7 @@ struct DecodePlan {
         nq = row_tiles = 0;
         px_rows = 0;
         const long long M = (long long)B * (n_q / n_kv);
+        size_t px_most = 0;
         // One sequence shares nothing, and less than two tiles of rows are not worth a launch of their own
         if (B > 1 && prefix >= 2 * TILE_ROWS) {
             nq = D == 256 || M <= TILE_ROWS ? 1 : 2;
@@ -171,14 +174,19 @@ struct DecodePlan {
             // longer than six tiles: the tensor cores cut sums off where fp32 arithmetic rounds, a stretch of t tiles
             // (16 t additions) loses up to 2.5e-8 per addition, and joining stretches does not (against 64 bits: 8,192 rows,
             // heads of 256, 1.7e-6; 32,768 rows, heads of 128, 1.4e-6; stretches of nine and of 37 tiles, which the waves
-            // alone would give, lost twice and eight times as much).
-            const int tiles = (prefix + TILE_ROWS - 1) / TILE_ROWS, base = n_kv * row_tiles;
-            const int least = f32 ? (tiles + 5) / 6 : 1;
+            // alone would give, lost twice and eight times as much). Beyond that, CTAs for four waves or eight per query tile
+            // at most, for scratch's sake (one in 180 of 40,000 drawn sizes would take more, by this count 11 % faster at best).
+            const int tiles = ((prefix < PagedKv::MOST_ROWS ? prefix : PagedKv::MOST_ROWS) + TILE_ROWS - 1) / TILE_ROWS;
+            const int six = (tiles + 5) / 6, least = f32 ? six : 1;
+            const long long base = (long long)n_kv * row_tiles, ctas = 4LL * sms > 8 * base ? 4LL * sms : 8 * base;
             long long best = LLONG_MAX;
-            for (int s = least; s <= tiles && s < least + 64; ++s) {
-                const long long cost = (((long long)base * s + sms - 1) / sms) * ((tiles + s - 1) / s + 4);
-                if (cost < best) { best = cost; splits = s; }
-            }
+            if (prefix <= PagedKv::MOST_ROWS)      // (no sequence has more)
+                for (int s = least; s <= tiles && s < least + 64 && (s == least || base * s <= ctas); ++s) {
+                    const long long cost = ((base * s + sms - 1) / sms) * ((tiles + s - 1) / s + 4);
+                    if (cost < best) { best = cost; splits = s; }
+                }
+            const long long longest = base * six > ctas ? base * six : ctas, all = base * tiles;
+            px_most = (size_t)(longest < all ? longest : all) * nq * TILE_ROWS;
         }
         const auto put = [this](size_t n) {
             const size_t at = bytes;
@@ -190,9 +198,8 @@ struct DecodePlan {
         shares = put((size_t)B * 4);
         own_ml = put(pieces * 8);
         own_o = put(pieces * D * 4);
-        const size_t px = (size_t)splits * n_kv * px_rows;
-        px_ml = put(px * 8);
-        px_o = put(px * D * 4);
+        px_ml = put(px_most * 8);
+        px_o = put(px_most * D * 4);
     }
 };
 
@@ -337,8 +344,7 @@ int b200_attn_gave_up(void) {
 
 size_t gpu_attn_decode_scratch_bytes(int n_q, int n_kv, int head_dim, int B, int prefix_len) {
     if (!good_heads(n_q, n_kv, head_dim) || B < 1 || (long long)B * n_q > (1 << 28) || prefix_len < 0) return 0;
-    const size_t a = DecodePlan(n_q, n_kv, head_dim, B, prefix_len, true).bytes, b = DecodePlan(n_q, n_kv, head_dim, B, prefix_len, false).bytes;
-    return a > b ? a : b;      // (serves both row types)
+    return DecodePlan(n_q, n_kv, head_dim, B, prefix_len, true).bytes;
 }
 
 cudaError_t gpu_attn_decode(const float* q, const uint16_t* K, const uint16_t* V, int kv_stride, int kv_shift, long long kv_bstride,

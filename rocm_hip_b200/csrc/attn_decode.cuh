@@ -20,9 +20,10 @@ struct PagedKv {
     const int* lens;    // [B]
     long long kv_bstride;
     int kv_stride, kv_shift, n_pages, max_pages;
-    // rows of sequence b: lens[b] within what its page list can hold (and a little below 2^31, so that whole tiles fit an int)
+    static constexpr int MOST_ROWS = INT_MAX - 4096;      // of a sequence: whole tiles fit an int
+    // rows of sequence b: lens[b] within what its page list can hold
     __device__ __forceinline__ int len(int b) const {
-        const long long cap = min((long long)max_pages << kv_shift, (long long)INT_MAX - 4096);
+        const long long cap = min((long long)max_pages << kv_shift, (long long)MOST_ROWS);
         const long long n = max(lens[b], 0);
         return (int)(n < cap ? n : cap);
     }

@@ -104,3 +104,30 @@ def test_struct_layout(tmp_path):
     subprocess.run(["gcc", "-I", os.path.join(root, "include"), "-I/usr/local/cuda/include", str(src), "-o", str(exe)], check=True)
     got = [int(x) for x in subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split()]
     assert got == [C.sizeof(_lib.b200_kv_pages)] + [getattr(_lib.b200_kv_pages, f).offset for f in fields]
+
+
+@pytest.mark.parametrize("n_q,n_kv,D", [(16, 4, 256), (16, 8, 128), (40, 8, 128), (8, 1, 64), (5, 1, 128), (128, 16, 256), (64, 2, 64)])
+def test_scratch_of_the_largest_call_serves_the_smaller_ones(lib, n_q, n_kv, D):
+    """One workspace for the largest batch behind the longest prefix: every call with fewer sequences or a shorter prefix takes it."""
+    Bs = sorted({*range(1, 40), *range(120, 135), 200, 255, 256, 257, 300, 511, 512, 1000})
+    prefixes = sorted({0, 16, 240, 256, 272, 1024, 2432, 8192, 8208, 16384, 32768, 131072, *range(256, 5000, 208)})
+    need = [[lib.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, B, p) for p in prefixes] for B in Bs]
+    for i, row in enumerate(need):
+        for j, n in enumerate(row):
+            assert n > 0 and (i == 0 or need[i - 1][j] <= n) and (j == 0 or row[j - 1] <= n), (Bs[i], prefixes[j])
+    kw = dict(DECODE, n_q=n_q, n_kv=n_kv, head_dim=D, kv_stride=n_kv * D, kv_bstride=32 * n_kv * D, max_pages=1 << 20)
+    for B, p in ((257, 8192), (129, 2432), (1000, 131072)):
+        most = lib.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, B, p)
+        for b in Bs:
+            for q in prefixes:
+                if b <= B and q <= p:
+                    for name in ("gpu_attn_decode", "gpu_attn_decode_bf16"):
+                        assert getattr(lib, name)(*dict(kw, B=b, prefix_len=q, scratch_bytes=most).values()) == NODEV, (B, p, b, q)
+    assert lib.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, 8, 2**31 - 1) >= lib.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, 8, 2**31 - 6000)
+
+
+def test_prefixes_beyond_what_a_sequence_can_hold(lib):
+    """Prefixes up to the largest int: allowed where the page lists can hold them, and never more than an int on the way."""
+    call = lambda **kw: lib.gpu_attn_decode(*{**DECODE, **kw}.values())  # noqa: E731
+    for shift, prefix in ((0, 2**31 - 1), (0, 2**31 - 128), (0, 2**31 - 4097), (0, 2**31 - 4095), (7, 2**31 - 128), (30, 2**30)):
+        assert call(kv_shift=shift, prefix_len=prefix, max_pages=2**31 - 1 >> shift) == NODEV, (shift, prefix)
