@@ -53,13 +53,33 @@ def _stream():
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def _stream_of(t):
-    """The current stream as an int, for the calls whose latency counts (a Stream object costs as much as a launch). The
-    launchers run on the current device: a tensor of another one is refused."""
+# The attention and KV-page calls are short enough for the host's part to count: pointers and streams go over as ints, and the
+# tensors are looked at in as few steps as it takes (each is a tenth of a microsecond).
+
+def _device():
+    """The current device, which the launchers run on, and its current stream as an int."""
     dev = torch.cuda.current_device()
+    return dev, torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _ints(what, t, n, dev):
+    """An index array of the launchers: int32, at least n of them in a row on device `dev`. Its address."""
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{what}: {t.dtype}, not int32")
+    if t.get_device() != dev or t.nbytes < 4 * n or not t.is_contiguous():
+        raise ValueError(f"{what}: {tuple(t.shape)} on {t.device}, {n} contiguous values on cuda:{dev} needed")
+    return t.data_ptr()
+
+
+def _room(what, t, n, dev, contiguous=False):
+    """n bytes from t's first value on are memory of t's, on device `dev`; contiguous: of t itself, which lies in a row. Its
+    address."""
     if t.get_device() != dev:
-        raise ValueError(f"tensor on device {t.get_device()}, current device {dev}")
-    return torch._C._cuda_getCurrentRawStream(dev)
+        raise ValueError(f"{what}: on {t.device}, current device {dev}")
+    if t.nbytes < n or not t.is_contiguous():
+        if contiguous or n > t.untyped_storage().nbytes() - t.storage_offset() * t.element_size():
+            raise ValueError(f"{what}: {tuple(t.shape)} in strides {t.stride()}, {n} bytes needed")
+    return t.data_ptr()
 
 
 def gpu_ops_init(co_path="gpu_ops.co"):
@@ -406,10 +426,16 @@ def gpu_attn_prompt(q, k, v, out, seq_start, n_seqs, T, n_q, n_kv, head_dim, sca
     n_seqs + 1 entries; None: one sequence of T rows). q, k, v, out: bfloat16 or float16 CUDA tensors."""
     if q.dtype not in (torch.bfloat16, torch.float16) or not (q.dtype == k.dtype == v.dtype == out.dtype):
         raise TypeError((q.dtype, k.dtype, v.dtype, out.dtype))
+    dev, stream = _device()
+    q_row, kv_row = n_q * head_dim, n_kv * head_dim
     lib = _lib.load()
-    fn = lib.gpu_attn_prompt_bf16 if q.dtype == torch.bfloat16 else lib.gpu_attn_prompt_f16
-    _check("gpu_attn_prompt", fn(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(seq_start), n_seqs, T, n_q, n_kv, head_dim, q_stride,
-                                 k_stride, v_stride, scale, _stream_of(q)))
+    fn = lib.gpu_attn_prompt_bf16 if q.dtype is torch.bfloat16 else lib.gpu_attn_prompt_f16
+    _check("gpu_attn_prompt", fn(_room("q", q, 2 * ((T - 1) * (q_stride or q_row) + q_row), dev, not q_stride),
+                                 _room("k", k, 2 * ((T - 1) * (k_stride or kv_row) + kv_row), dev, not k_stride),
+                                 _room("v", v, 2 * ((T - 1) * (v_stride or kv_row) + kv_row), dev, not v_stride),
+                                 _room("out", out, 2 * T * q_row, dev, True),
+                                 None if seq_start is None else _ints("seq_start", seq_start, n_seqs + 1, dev),
+                                 n_seqs, T, n_q, n_kv, head_dim, q_stride, k_stride, v_stride, scale, stream))
 
 
 def gpu_attn_decode_scratch_bytes(n_q, n_kv, head_dim, B, prefix_len=0):
@@ -420,17 +446,22 @@ def gpu_attn_decode(q, K, V, kv_stride, kv_shift, kv_bstride, n_pages, pages, ma
                     head_dim, B, scale, scratch=None):
     """Attention of one token per sequence over the paged FP16 cache K / V (float16 CUDA tensors, row 0 of page 0 of the
     layer's K and V). q, out: float32 or bfloat16 [B][n_q * head_dim]; pages int32 [B][max_pages]; lens int32 [B];
-    prefix_len: rows that all sequences share, read once. scratch: a CUDA tensor of gpu_attn_decode_scratch_bytes(...)
+    prefix_len: rows read once for the sequences whose page lists begin alike. scratch: a CUDA tensor of gpu_attn_decode_scratch_bytes(...)
     bytes (one is made when None)."""
     if q.dtype not in (torch.float32, torch.bfloat16) or q.dtype != out.dtype or K.dtype != torch.float16 or V.dtype != torch.float16:
         raise TypeError((q.dtype, out.dtype, K.dtype, V.dtype))
+    dev, stream = _device()
+    n = B * n_q * head_dim * (4 if q.dtype is torch.float32 else 2)
+    # (pages of more than 4,096 rows need not be memory to their end)
+    cache = 2 * ((n_pages - 1) * kv_bstride + ((1 << kv_shift) - 1) * kv_stride + n_kv * head_dim) if 0 <= kv_shift <= 12 else 0
     lib = _lib.load()
     if scratch is None:
         scratch = torch.empty(gpu_attn_decode_scratch_bytes(n_q, n_kv, head_dim, B, prefix_len), dtype=torch.uint8, device=q.device)
-    fn = lib.gpu_attn_decode if q.dtype == torch.float32 else lib.gpu_attn_decode_bf16
-    _check("gpu_attn_decode", fn(_ptr(q), _ptr(K), _ptr(V), kv_stride, kv_shift, kv_bstride, n_pages, _ptr(pages), max_pages, _ptr(lens),
-                                 prefix_len, _ptr(out), n_q, n_kv, head_dim, B, scale, _ptr(scratch),
-                                 scratch.numel() * scratch.element_size(), _stream_of(q)))
+    fn = lib.gpu_attn_decode if q.dtype is torch.float32 else lib.gpu_attn_decode_bf16
+    _check("gpu_attn_decode", fn(_room("q", q, n, dev, True), _room("K", K, cache, dev), _room("V", V, cache, dev), kv_stride, kv_shift,
+                                 kv_bstride, n_pages, _ints("pages", pages, B * max_pages, dev), max_pages, _ints("lens", lens, B, dev),
+                                 prefix_len, _room("out", out, n, dev, True), n_q, n_kv, head_dim, B, scale,
+                                 _room("scratch", scratch, 0, dev, True), scratch.nbytes, stream))
 
 
 class KvPages:
@@ -440,35 +471,49 @@ class KvPages:
 
     def __init__(self, table, lens, refs, info, page_shift, pool, page_bytes, n_parts=1, part_stride=0):
         n_seqs, max_pages = table.shape
-        for t, n in ((table, n_seqs * max_pages), (lens, n_seqs), (refs, refs.numel()), (info, 4)):
-            assert t.is_cuda and t.dtype == torch.int32 and t.is_contiguous() and t.numel() >= n
+        if not table.is_cuda:
+            raise ValueError(f"table on {table.device}")
+        for what, t, n in (("table", table, 0), ("lens", lens, n_seqs), ("refs", refs, 1), ("info", info, 4)):
+            _ints(what, t, n, table.get_device())
         n_pages = refs.numel()
-        assert pool.is_cuda and pool.numel() * pool.element_size() >= (n_parts - 1) * part_stride + n_pages * page_bytes
+        _room("pool", pool, (n_parts - 1) * part_stride + n_pages * page_bytes, table.get_device())
         self.work = torch.empty(int(_lib.load().gpu_kv_pages_work_ints(n_seqs, n_pages)), dtype=torch.int32, device=table.device)
         self.table, self.lens, self.refs, self.info, self.pool = table, lens, refs, info, pool
         p = lambda t: t.data_ptr()  # noqa: E731
         self._struct = _lib.b200_kv_pages(p(table), p(lens), p(refs), p(info), p(self.work), n_seqs, max_pages, n_pages, page_shift,
                                           p(pool), page_bytes, n_parts, part_stride)
 
+        self.struct_ref, self.n_seqs, self.device = C.byref(self._struct), n_seqs, table.get_device()
+
     def struct(self):
         return self._struct
+
+    def stream(self):
+        """The current device, which has to be the tables', and its current stream."""
+        dev, stream = _device()
+        if dev != self.device:
+            raise ValueError(f"tables on device {self.device}, current device {dev}")
+        return dev, stream
 
 
 def gpu_kv_pages_fork(kv, parent):
     """parent int32 [n_seqs]: -1, or the sequence that the empty sequence s becomes a copy of."""
-    _check("gpu_kv_pages_fork", _lib.load().gpu_kv_pages_fork(C.byref(kv.struct()), _ptr(parent), _stream_of(kv.table)))
+    dev, stream = kv.stream()
+    _check("gpu_kv_pages_fork", _lib.load().gpu_kv_pages_fork(kv.struct_ref, _ints("parent", parent, kv.n_seqs, dev), stream))
 
 
 def gpu_kv_pages_resize(kv, new_lens, slots=None):
     """new_lens int32 [n_seqs]: the length each sequence gets (0 frees it, negative keeps it); slots (int32): receives the
     cache rows of the new tokens."""
-    _check("gpu_kv_pages_resize", _lib.load().gpu_kv_pages_resize(C.byref(kv.struct()), _ptr(new_lens), _ptr(slots),
-                                                                  0 if slots is None else slots.numel(), _stream_of(kv.table)))
+    dev, stream = kv.stream()
+    _check("gpu_kv_pages_resize", _lib.load().gpu_kv_pages_resize(kv.struct_ref, _ints("new_lens", new_lens, kv.n_seqs, dev),
+                                                                  None if slots is None else _ints("slots", slots, 0, dev),
+                                                                  0 if slots is None else slots.numel(), stream))
 
 
 def gpu_kv_pages_compact(kv):
     """Moves the pages in use to the lowest ids."""
-    _check("gpu_kv_pages_compact", _lib.load().gpu_kv_pages_compact(C.byref(kv.struct()), _stream_of(kv.table)))
+    _check("gpu_kv_pages_compact", _lib.load().gpu_kv_pages_compact(kv.struct_ref, kv.stream()[1]))
 
 
 class HostRows:
