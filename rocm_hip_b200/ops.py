@@ -14,7 +14,7 @@ from . import _lib
 __all__ = [
     "LayerOpError", "gpu_ops_init", "gpu_ops_free", "gpu_add_rmsnorm", "gpu_swiglu", "gpu_swiglu_rows",
     "gpu_qk_norm_rope", "gpu_rope_table", "gpu_qk_norm_rope_tab", "gpu_qk_norm_rope_tab_kv", "gpu_qk_norm_rope_kv", "gpu_attn_prep_f16", "gpu_embed_rows", "gpu_moe_group", "gpu_moe_group_scratch_ints", "gpu_moe_max_tiles", "gpu_kv_store_f16", "gpu_kv_store_q", "gpu_hadamard_rot", "gpu_add_normed", "gpu_gemma_attn_post", "gpu_geglu", "gpu_softcap", "gpu_gemma_ffn_post", "gpu_moe_combine", "gpu_moe_router", "gpu_moe_router_sigmoid", "gpu_relu2", "gpu_mamba_conv", "gpu_mamba_scan", "gpu_ple_conv", "gpu_hc_norm", "gpu_hc_lowrank", "gpu_hc_mix", "gpu_ple_gate", "gpu_mtp_concat", "gpu_mamba_gnorm", "gpu_rmsnorm_f16", "gpu_rope_rotate_half_f16", "launch_count", "Q8Buffers",
-    "gpu_attn_prompt", "gpu_attn_decode", "gpu_attn_decode_scratch_bytes", "KvPages", "gpu_kv_pages_fork",
+    "gpu_attn_prompt", "gpu_attn_decode", "attn_gave_up", "gpu_attn_decode_scratch_bytes", "KvPages", "gpu_kv_pages_fork",
     "gpu_kv_pages_resize", "gpu_kv_pages_compact",
     "QT_Q4_0", "QT_Q8_0", "QT_F32", "QT_F16", "QT_BF16", "QT_Q4_1", "QT_Q5_0", "QT_Q5_1", "QT_Q4_K", "QT_Q5_K", "QT_Q6_K",
     "QT_BLOCKS", "qt_row_size", "HostRows", "HostGroup",
@@ -92,6 +92,16 @@ def gpu_ops_free():
 
 def launch_count():
     return int(_lib.load().b200_launch_count())
+
+
+def attn_gave_up():
+    """How many blocks of the attention kernels have given up on a wait on the current device since the library was loaded (0 in
+    sound operation; the rows of such a block are unspecified, and the call that launched it has returned without an error).
+    Waits for the device; raises when the count cannot be had."""
+    n = int(_lib.load().b200_attn_gave_up())
+    if n < 0:
+        raise LayerOpError("b200_attn_gave_up", n)
+    return n
 
 
 class Q8Buffers:

@@ -5,5 +5,4 @@ pytestmark = pytest.mark.gpu
 
 
 def test_no_block_gave_up(ops):
-    from rocm_hip_b200 import _lib
-    assert _lib.load().b200_attn_gave_up() == 0
+    assert ops.attn_gave_up() == 0
