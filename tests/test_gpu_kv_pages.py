@@ -322,3 +322,45 @@ def test_many_sequences_cut_back_at_once(ops, n_seqs):
         x.resize([r.randint(0, n) if r.random() < 0.9 else -1 for n in x.m.lens])
     x.resize([0] * n_seqs)
     assert x.m.info[1] == n_pages
+
+
+def test_single_tokens_as_the_integration_notes_have_them(ops):
+    """Pages for one more token, its K row normed, rotated and written into the cache by one call, its V row by another, the
+    attention from the cache: step after step against 64 bits."""
+    from test_gpu_attention import attend, check
+    n_q, n_kv, D, shift, n_seqs, max_pages, n_pages = 8, 2, 128, 3, 5, 12, 50
+    page, kv, scale, G = 1 << shift, n_kv * D, D ** -0.5, n_q // n_kv
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rnd = lambda *n: torch.randn(*n, generator=g, device="cuda")  # noqa: E731
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device="cuda")  # noqa: E731
+    pool = torch.full((n_pages, 2, page, kv), float("nan"), dtype=torch.float16, device="cuda")
+    pages = ops.KvPages(torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device="cuda"), z(n_seqs), z(n_pages), z(4), shift, pool,
+                        2 * page * kv * 2)
+    qn, kn = 1 + 0.1 * rnd(D), 1 + 0.1 * rnd(D)
+    history = [[] for _ in range(n_seqs)]      # (k rotated by the call that returns it, v) as the cache holds them
+    slots, ct, sn = z(n_seqs), torch.empty(n_seqs, D // 2, device="cuda"), torch.empty(n_seqs, D // 2, device="cuda")
+    for step in range(20):
+        q, k, v = (rnd(n_seqs, w * D).bfloat16() for w in (n_q, n_kv, n_kv))
+        ops.gpu_kv_pages_resize(pages, ints([step + 1] * n_seqs), slots)
+        ops.gpu_rope_table(ints([step] * n_seqs), 0, n_seqs, D, 0, 1e6, ct, sn)
+        q_rot, q_ref, k_ref = torch.empty_like(q), torch.empty_like(q), torch.empty_like(k)
+        ops.gpu_qk_norm_rope_tab_kv(q, k, qn, kn, q_rot, pool[0, 0], kv, shift, 2 * page * kv, n_q, n_kv, D, D, ct, sn, slots, 0, n_seqs, 1e-6)
+        ops.gpu_kv_store_f16(v, pool[0, 1], kv, slots, 0, n_seqs, kv, shift, 2 * page * kv)
+        out = torch.empty_like(q)
+        ops.gpu_attn_decode(q_rot, pool, pool[0, 1], kv, shift, 2 * page * kv, n_pages, pages.table, max_pages, pages.lens, 0, out, n_q, n_kv, D,
+                            n_seqs, scale)
+        ops.gpu_qk_norm_rope_tab(q, k, qn, kn, q_ref, k_ref, n_q, n_kv, D, D, ct, sn, n_seqs, 1e-6)
+        assert torch.equal(q_rot, q_ref)
+        for s in range(n_seqs):
+            row = pool[slots[s] // page, :, slots[s] % page]
+            # (K goes from fp32 to fp16 in the fused call: half a step of either type apart from the bf16 row)
+            assert ((row[0].float() - k_ref[s].float()).abs() <= (2.0**-8 + 2.0**-11) * 1.01 * k_ref[s].float().abs() + 2.0**-24).all()
+            assert torch.equal(row[1], v[s].half())
+            history[s].append((row[0].clone(), row[1].clone()))
+            K, V = (torch.stack([x[i] for x in history[s]]).double() for i in (0, 1))
+            for h in range(n_kv):
+                see = torch.ones(G, step + 1, dtype=torch.bool, device="cuda")
+                want, bound = attend(q_rot[s].double().view(n_kv, G, D)[h], K[:, h * D:(h + 1) * D], V[:, h * D:(h + 1) * D], see, scale,
+                                     torch.float16)
+                check(out[s].view(n_kv, G, D)[h], want, bound, torch.bfloat16)
