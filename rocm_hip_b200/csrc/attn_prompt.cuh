@@ -230,7 +230,7 @@ k_attn_prompt(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CU
                     }
                     const int b = max(lo - 1, 0);
                     first = min(max(seq_start[b], 0), rows);
-                    end = min(seq_start[b + 1], rows);
+                    end = max(first, min(seq_start[b + 1], rows));
                     tile = slot - (first / ROWS + b);
                 }
                 if (tile >= 0 && tile <= (end - first) / ROWS && first + tile * ROWS < end) {   // (no overflow on bad borders)
