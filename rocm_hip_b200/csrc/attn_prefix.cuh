@@ -154,7 +154,9 @@ k_attn_prefix(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CU
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int x = q_exponent(top);
-            const float k0 = pow2(x / 2), k1 = pow2(x - x / 2), c = __shfl_sync(0xffffffffu, scale2e(scale2, -x), (lane & 7) * 4);
+            // (c > 0 also for a row near the least float: a hidden score, -inf, times 0 would be NaN)
+            const float k0 = pow2(x / 2), k1 = pow2(x - x / 2), c_own = fmaxf(scale2e(scale2, -x), 0x1p-126f);
+            const float c = __shfl_sync(0xffffffffu, c_own, (lane & 7) * 4);
             if (lane >> 3 == r8 >> 3) c_row = c;
             unsigned char* row = smem + i * Ti::QTILE * (SPLIT ? 2 : 1) + in_tile * 128;
 #pragma unroll

@@ -3,7 +3,7 @@ lengths. Against 64 bits with the bounds of test_gpu_attention.py."""
 import pytest
 import torch
 
-from test_gpu_attention import BF, F32, decode, decode_check, paged
+from test_gpu_attention import BF, F16, F32, attend, check, decode, decode_check, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -83,3 +83,27 @@ def test_captured_call_follows_the_lists(ops):
         scratch.fill_(0xff)
         graph.replay()
         decode_check(out, q, pool, table, L, page, n_q, n_kv, D, 0.1)
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("size,scale", [(1e-38, 1e-6), (1e-38, 0.1), (1e-30, 1e-30), (5e37, 1e-37), (1e30, 1e-30)])
+def test_queries_near_the_ends_of_the_range(ops, size, scale, D, dt):
+    """Queries near the least and the largest float, a page of the prefix that nobody sees and one of a sequence's own."""
+    lens, n_q, n_kv, page, prefix = [300, 257, 700, 256], 4, 2, 16, 256
+    pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 34)
+    table[:, 3] = -1
+    table[2, 20] = n_pages
+    q = (queries(4, n_q, D, F32) * size).to(dt)
+    assert torch.isfinite(q).all()
+    out = decode(ops, q, pool, table, L, stride, n_pages, max_pages, page, prefix, n_q, n_kv, D, scale)
+    for b in range(4):
+        t = torch.arange(lens[b], device="cuda")
+        p = table[b].long()[t // page]
+        seen = (p >= 0) & (p < n_pages)
+        rows = pool[p[seen], :, (t % page)[seen], :n_kv * D]
+        for h in range(n_kv):
+            k, v = (rows[:, i, h * D:(h + 1) * D].double() for i in (0, 1))
+            see = torch.ones(2, k.shape[0], dtype=torch.bool, device="cuda")
+            want, bound = attend(q[b].double().view(n_kv, 2, D)[h], k, v, see, scale, F16 if dt == BF else None)
+            check(out[b].view(n_kv, 2, D)[h], want, bound, dt)
