@@ -89,7 +89,10 @@ struct Tiles {
     // 32 heads of 128: 1,246 -> 1,295 TFLOP/s). With one query tile the next S fills that time (heads of 256: 1,286 without,
     // 1,261 with).
     static constexpr bool HALVES = NQ == 2;
-    static constexpr int P_SHIFT_T = std::is_same<T, __half>::value ? 7 : 0;   // fp16 weights are held times 2^7 (at most 2^15)
+    // Weights are held times a power of two: fp16 ones 2^7 (at most 2^15, and normal for as long as they count), bf16 ones
+    // 2^-24: m may lag by 2^8, so the sum of 65,536 of them is at most 1 and finite v of any size cannot make O overflow,
+    // while v of 1e-30 still give normal products.
+    static constexpr int P_SHIFT_T = std::is_same<T, __half>::value ? 7 : -24;
 
     // A softmax thread holds its row's 128 scores: 224 registers. Twelve warps start with 168 each (64,512 in all); the four
     // that compute nothing go down to 56 and the eight softmax warps up, 4 x 32 x 56 + 8 x 32 x 224 = 64,512. (Seven
@@ -345,7 +348,7 @@ struct Tiles {
             f2 w = fma2(pk2(__uint_as_float(x[at]), __uint_as_float(x[at + 1])), c2, neg2);
             float a, b;
             if (EMU && e % (EMU + !EMU) == EMU - 1) {
-                w = ex2_poly<P_SHIFT_T ? 4 : 3>(w);
+                w = ex2_poly<std::is_same<T, __half>::value ? 4 : 3>(w);
                 upk2(w, a, b);
             } else {
                 upk2(w, a, b);

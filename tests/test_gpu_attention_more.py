@@ -96,3 +96,34 @@ def test_large_pages_behind_a_prefix(ops, page, D, dt):
     q = torch.randn(len(lens), n_q * D, generator=torch.Generator(device="cuda").manual_seed(46), device="cuda").to(dt)
     out = decode(ops, q, pool, table, L, stride, n_pages, max_pages, page, page, n_q, n_kv, D, 0.1)
     decode_check(out, q, pool, table, L, page, n_q, n_kv, D, 0.1)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n_q,n_kv,lens", [(2, 1, [300]), (16, 8, LENS), (15, 5, LENS)])
+def test_large_values(ops, D, n_q, n_kv, lens):
+    """v near 1e36, a 340th of the largest float, behind scores that rise by less than the factor 2^8 that a running maximum may
+    lag by."""
+    q, k, v, starts, ss = prompt_inputs(lens, n_q, n_kv, D, BF, 47)
+    q.fill_(1.0)
+    rise = torch.zeros(q.shape[0], 1, device="cuda")
+    for a, b in zip(starts, starts[1:]):
+        rise[a + 128:b] = 5.0
+    k.copy_((rise / (0.1 * D) + 0.001 * k.float()).to(BF))
+    v.copy_((v.float().abs() * 1e36).to(BF))
+    out = torch.empty_like(q)
+    ops.gpu_attn_prompt(q, k, v, out, ss, len(lens), q.shape[0], n_q, n_kv, D, 0.1)
+    prompt_check(q, k, v, out, starts, n_q, n_kv, D, 0.1, BF)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("n_q,n_kv", [(2, 1), (16, 8), (15, 5)])
+@pytest.mark.parametrize("size", [2.0**126, 2.0**-96])
+def test_values_near_the_ends_of_the_range(ops, D, n_q, n_kv, size):
+    """v within a factor of two of the largest bf16 value, all of one sign, and near 1e-29."""
+    q, k, v, starts, ss = prompt_inputs(LENS, n_q, n_kv, D, BF, 48)
+    v.copy_(((1 + torch.rand(v.shape, generator=torch.Generator(device="cuda").manual_seed(48), device="cuda")) * 0.99 * size).to(BF))
+    assert torch.isfinite(v).all()
+    out = torch.empty_like(q)
+    ops.gpu_attn_prompt(q, k, v, out, ss, len(LENS), q.shape[0], n_q, n_kv, D, 0.1)
+    # (64-bit values and bounds of v / size: powers of two change no rounding here)
+    prompt_check(q, k, v / size, (out.double() / size).float(), starts, n_q, n_kv, D, 0.1, BF)
