@@ -58,7 +58,7 @@ def _stream():
 
 def _device():
     """The current device, which the launchers run on, and its current stream as an int."""
-    dev = torch.cuda.current_device()
+    dev = torch._C._cuda_getDevice()
     return dev, torch._C._cuda_getCurrentRawStream(dev)
 
 
