@@ -233,7 +233,7 @@ cudaError_t launch_decode_d(const T* q, const PagedKv& kv, int prefix, T* out, i
         static std::atomic<unsigned long long> done;                                                                         \
         if ((st = allow_smem(k_attn_own<D, T, BOX_>, OwnShape<D>::SMEM, done)) != cudaSuccess) return st;                         \
         launch_pdl((k_attn_own<D, T, BOX_>), (unsigned)pl.grid_own, OwnShape<D>::WARPS * 32, OwnShape<D>::SMEM, stream, ok, ov, q, kv, \
-                   sc, own, n_q, n_q / n_kv, B, behind, scale2, 2);                                                                    \
+                   sc, own, n_q, n_q / n_kv, B, behind, scale2);                                                                       \
     } while (0)
     if (box) OWN(true); else OWN(false);
 #undef OWN

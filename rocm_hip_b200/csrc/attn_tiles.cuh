@@ -8,6 +8,10 @@
 // rescaled only when a row's maximum has grown by more than 2^8 since it was last taken: P then stays within what
 // 16-bit floats and the fp32 sums bear, and almost no tile after the first pays for reading and writing O. Rounding P to
 // 16 bits is what the tensor cores take (SPLIT: P = hi + lo, 22 bits, two products; Q likewise); l sums unrounded values.
+//
+// The methods are published ones: softmax with a running maximum and sum (Milakov and Gimelshein, 2018, "Online normalizer
+// calculation for softmax"), two query tiles that take turns at the tensor cores, O rescaled only past a threshold, part of the
+// exponentials by a polynomial after Cody and Waite's range reduction. The code and the coefficients are this library's own.
 
 #ifndef B200_ATTN_TILES_CUH
 #define B200_ATTN_TILES_CUH

@@ -127,3 +127,30 @@ def test_values_near_the_ends_of_the_range(ops, D, n_q, n_kv, size):
     ops.gpu_attn_prompt(q, k, v, out, ss, len(LENS), q.shape[0], n_q, n_kv, D, 0.1)
     # (64-bit values and bounds of v / size: powers of two change no rounding here)
     prompt_check(q, k, v / size, (out.double() / size).float(), starts, n_q, n_kv, D, 0.1, BF)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("prefix", [0, 256])
+def test_scores_of_minus_infinity_over_a_cache(ops, prefix, D):
+    """bf16 rows: keys whose scores are -inf carry no weight; a sequence that sees nothing else is zero. Others are as without."""
+    lens, n_q, n_kv, page = [300, 290, 270, 400], 4, 2, 16
+    pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 49)
+    q = torch.randn(4, n_q * D, generator=torch.Generator(device="cuda").manual_seed(49), device="cuda").abs().add(0.1).to(BF)
+    args = (q, pool, table, L, stride, n_pages, max_pages, page, prefix, n_q, n_kv, D, 0.1)
+    clean = decode(ops, *args)
+    rows = lambda b, t: (table[b].long()[t // page], t % page)  # noqa: E731
+    t = torch.arange(lens[3], device="cuda")
+    p, r = rows(3, t[256 if prefix else 0:][::3])         # a third of what only the last sequence sees
+    pool[p, 0, r] = -float("inf")
+    out = decode(ops, *args)
+    assert torch.equal(out[:3], clean[:3])
+    seen = torch.ones_like(t, dtype=torch.bool)
+    seen[(256 if prefix else 0)::3] = False
+    p, r = rows(3, t[seen])
+    x = pool[p, :, r, :n_kv * D]
+    for h in range(n_kv):
+        k, v = (x[:, i, h * D:(h + 1) * D].double() for i in (0, 1))
+        want, bound = attend(q[3].double().view(n_kv, 2, D)[h], k, v, torch.ones(2, k.shape[0], dtype=torch.bool, device="cuda"), 0.1, F16)
+        check(out[3].view(n_kv, 2, D)[h], want, bound, BF)
+    pool[:, 0] = -float("inf")
+    assert (decode(ops, *args) == 0).all()
