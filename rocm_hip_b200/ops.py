@@ -458,17 +458,21 @@ def gpu_attn_decode(q, K, V, kv_stride, kv_shift, kv_bstride, n_pages, pages, ma
     layer's K and V). q, out: float32 or bfloat16 [B][n_q * head_dim]; pages int32 [B][max_pages]; lens int32 [B];
     prefix_len: rows read once for the sequences whose page lists begin alike. scratch: a CUDA tensor of gpu_attn_decode_scratch_bytes(...)
     bytes (one is made when None)."""
-    if q.dtype not in (torch.float32, torch.bfloat16) or q.dtype != out.dtype or K.dtype != torch.float16 or V.dtype != torch.float16:
+    dt = q.dtype
+    if (dt is not torch.float32 and dt is not torch.bfloat16) or out.dtype is not dt or K.dtype is not torch.float16 or V.dtype is not torch.float16:
         raise TypeError((q.dtype, out.dtype, K.dtype, V.dtype))
     dev, stream = _device()
-    n = B * n_q * head_dim * (4 if q.dtype is torch.float32 else 2)
+    n = B * n_q * head_dim * (4 if dt is torch.float32 else 2)
     # (pages of more than 4,096 rows need not be memory to their end)
     cache = 2 * ((n_pages - 1) * kv_bstride + ((1 << kv_shift) - 1) * kv_stride + n_kv * head_dim) if 0 <= kv_shift <= 12 else 0
     lib = _lib.load()
     if scratch is None:
         scratch = torch.empty(gpu_attn_decode_scratch_bytes(n_q, n_kv, head_dim, B, prefix_len), dtype=torch.uint8, device=q.device)
-    fn = lib.gpu_attn_decode if q.dtype is torch.float32 else lib.gpu_attn_decode_bf16
-    _check("gpu_attn_decode", fn(_room("q", q, n, dev, True), _room("K", K, cache, dev), _room("V", V, cache, dev), kv_stride, kv_shift,
+    fn = lib.gpu_attn_decode if dt is torch.float32 else lib.gpu_attn_decode_bf16
+    # (V, as a rule, is the view of K's pool that its pages' other halves are: what holds for K's pages holds for it)
+    inside = V.get_device() == dev and not V.is_contiguous()
+    _check("gpu_attn_decode", fn(_room("q", q, n, dev, True), _room("K", K, cache, dev),
+                                 V.data_ptr() if inside else _room("V", V, cache, dev), kv_stride, kv_shift,
                                  kv_bstride, n_pages, _ints("pages", pages, B * max_pages, dev), max_pages, _ints("lens", lens, B, dev),
                                  prefix_len, _room("out", out, n, dev, True), n_q, n_kv, head_dim, B, scale,
                                  _room("scratch", scratch, 0, dev, True), scratch.nbytes, stream))
