@@ -107,3 +107,72 @@ def test_queries_near_the_ends_of_the_range(ops, size, scale, D, dt):
             see = torch.ones(2, k.shape[0], dtype=torch.bool, device="cuda")
             want, bound = attend(q[b].double().view(n_kv, 2, D)[h], k, v, see, scale, F16 if dt == BF else None)
             check(out[b].view(n_kv, 2, D)[h], want, bound, dt)
+
+
+@pytest.mark.parametrize("D,n_q,n_kv", [(64, 8, 2), (128, 16, 8), (128, 5, 1), (256, 16, 4)])
+def test_one_scratch_for_all_sizes(ops, D, n_q, n_kv):
+    """The scratch of the largest call, full of NaN, under smaller ones; nothing behind what a call asks for is written."""
+    page, sizes = 16, [(40, 2048), (129, 512), (3, 4096), (130, 256), (17, 1040), (1, 2048), (64, 0), (2, 272)]
+    most = ops.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, 130, 4096)
+    guard = 1 << 16
+    buf = torch.empty(most + guard, dtype=torch.uint8, device="cuda")
+    for B, prefix in sizes:
+        lens = [prefix + (11 * i) % 70 + 1 for i in range(B)]
+        pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 35)
+        need = ops.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, B, prefix)
+        assert need <= most
+        for dt in (F32, BF):
+            q = queries(B, n_q, D, dt)
+            for size in (need, most):
+                buf.fill_(0xff)
+                out = torch.full_like(q, float("nan"))
+                ops.gpu_attn_decode(q, pool, pool[0, 1], stride, 4, 2 * page * stride, n_pages, table, max_pages, L, prefix, out, n_q, n_kv, D,
+                                    B, 0.1, buf[:size])
+                assert (buf[need:] == 0xff).all()
+                decode_check(out[:20], q[:20], pool, table, L, page, n_q, n_kv, D, 0.1)
+                assert torch.isfinite(out).all()
+
+
+def test_a_scratch_and_lists_of_two_captured_calls(ops):
+    """Two captured calls of different sizes that share one scratch, replayed in turn on one stream; two with their own, on two."""
+    D, page, n_q, n_kv = 128, 16, 8, 2
+    made = []
+    most = max(ops.gpu_attn_decode_scratch_bytes(n_q, n_kv, D, B, p) for B, p in ((70, 512), (9, 1024)))
+    shared = torch.empty(most, dtype=torch.uint8, device="cuda")
+    for B, prefix, dt in ((70, 512, F32), (9, 1024, BF)):
+        lens = [prefix + 5 * i for i in range(B)]
+        pool, table, L, stride, n_pages, max_pages = paged(lens, n_kv, D, page, prefix, 36 + B)
+        q = queries(B, n_q, D, dt)
+        out, own = torch.empty_like(q), torch.empty(most, dtype=torch.uint8, device="cuda")
+        graphs = []
+        for scratch in (shared, own):
+            call = lambda: ops.gpu_attn_decode(q, pool, pool[0, 1], stride, 4, 2 * page * stride, n_pages, table, max_pages, L, prefix, out,  # noqa: E731,B023
+                                               n_q, n_kv, D, B, 0.1, scratch)  # noqa: B023
+            call()
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                call()
+            graphs.append(g)
+        call()
+        torch.cuda.synchronize()
+        # (a capture empties the allocator's cache: whatever a graph reads has to be kept)
+        made.append((graphs, out, out.clone(), (pool, table, L, q, own)))
+    for _ in range(5):
+        for _, out, _, _ in made:
+            out.fill_(float("nan"))
+        for graphs, _, _, _ in made:
+            graphs[0].replay()
+        for _, out, want, _ in made:
+            assert torch.equal(out, want)
+    side = [torch.cuda.Stream() for _ in made]
+    for _ in range(5):
+        for _, out, _, _ in made:
+            out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for s, (graphs, _, _, _) in zip(side, made):
+            with torch.cuda.stream(s):
+                graphs[1].replay()
+        torch.cuda.synchronize()
+        for _, out, want, _ in made:
+            assert torch.equal(out, want)
